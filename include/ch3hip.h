@@ -277,6 +277,56 @@ int h3hip_qkv_proj(const void* x, int64_t ldx, const void* w, int64_t ldw, int32
 int h3hip_out_proj(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t in_features,
                    int32_t out_features, int32_t seq_len, void* y, int64_t ldy, void* stream);
 
+/* ------------------------------------------------------- int8 projections */
+
+/* Rows of bf16 rounded to int8 with one scale a row, the operands of the int8
+ * projections: activations on every call, weights once. No counterpart in the
+ * reference, whose projections are bf16 matmuls (DiTBlock.swift:336-359).
+ *   a = max_k |x[m, k]|, q[m, k] = 127 x[m, k] / a rounded half to even (exactly: no
+ *   quotient is rounded before), scale[m] = a / 127 in fp32, so that x is about
+ *   q * scale. A row of zeros has scale 0. A row that holds an infinity or a NaN has
+ *   scale NaN and values 0: every product with it is NaN.
+ *   x:     device bf16 [rows, cols], row stride ldx elements, any alignment (rows on
+ *          16 bytes, i.e. x 16-byte aligned and ldx a multiple of 8, load widest).
+ *   q:     device int8 [rows, cols_pad], cols_pad = ceil(cols/128)*128, row stride
+ *          ldq bytes (a multiple of 16); 16-byte aligned; columns past cols are zeros.
+ *   scale: device fp32 [rows].
+ * rows may be 0. No workspace; can be captured into a graph. */
+int h3hip_quant_rows(const void* x, int64_t ldx, int32_t rows, int32_t cols, void* q, int64_t ldq,
+                     float* scale, void* stream);
+
+/* A projection on int8 operands with scales for each token and channel:
+ *   y[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n]
+ * The sum is exact (int32); it, and its products with the scales, are rounded to
+ * fp32, the result once to bf16. The int8 form of h3hip_out_proj, for any number of
+ * rows (0 and 1 too) and any width.
+ *   x: device int8 [rows, in_features], row stride ldx bytes; w: device int8
+ *      [out_features, in_features], row stride ldw bytes: as h3hip_quant_rows writes
+ *      them (any values, -128 too; 16-byte aligned, strides multiples of 16).
+ *   x_scale: device fp32 [rows]; w_scale: device fp32 [out_features], 16-byte aligned.
+ *   y: device bf16 [rows, out_features], row stride ldy elements; nothing else is
+ *      written. Any alignment (16 bytes and ldy a multiple of 8 store widest).
+ * Operands may pass 4 GiB; 256 rows of x or w must stay below 2 GiB.
+ * Declines unless in_features is a multiple of 128 (h3hip_quant_rows pads with
+ * zeros) and at most 131,071. No workspace; can be captured into a graph. */
+int h3hip_proj_i8(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
+                  const float* w_scale, int32_t in_features, int32_t out_features, int32_t rows,
+                  void* y, int64_t ldy, void* stream);
+
+/* h3hip_qkv_proj on int8 operands: the product of h3hip_proj_i8 for Q | K | V rows of
+ * w, rounded to bf16, with the head norm and the rotation in its epilogue. Q and K come
+ * out equal, bit for bit, to h3hip_qk_norm_rope applied to h3hip_proj_i8's result; V is
+ * that result, head-major.
+ *   x, x_scale, w, w_scale: as for h3hip_proj_i8, w [3*heads*head_dim, hidden].
+ *   Everything else as for h3hip_qkv_proj (both gammas NULL: the plain product, head-major).
+ * Declines unless head_dim == 128, rot is 96 or 128 and hidden is a multiple of 128 of
+ * at most 131,071; any head count. */
+int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
+                      const float* w_scale, int32_t hidden, const void* q_gamma,
+                      const void* k_gamma, float eps, const void* rope_table, int32_t rot,
+                      int32_t rounding, int32_t seq_len, int32_t seq_pad, int32_t heads,
+                      int32_t head_dim, void* q_out, void* k_out, void* v_out, void* stream);
+
 /* -------------------------------------------------------------- attention */
 
 /* Block-sparse attention over the plan's active tiles: for each query row,

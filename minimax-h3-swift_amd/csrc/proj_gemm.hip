@@ -27,11 +27,9 @@
 // code (norm_rope.h) and the render's rotation table. Rows that are complete
 // run without a branch so that two passes overlap: one wave per SIMD has no
 // other to cover its latencies.
-#include <type_traits>
-
 #include "gemm_loop.inc"
-#include "norm_rope.h"
 #include "proj.h"
+#include "proj_rows.h"
 #include "tile_order.h"
 
 namespace h3hip {
@@ -95,7 +93,6 @@ __device__ __forceinline__ void finish_tile(const ProjArgs& a, uint16_t* lds,
                                             int m0, int n0) {
   constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
   const int wc = wave >> 1, wt = wave & 1, lr = lane & 15, g = lane >> 4;
-  const int inner = a.heads * kHead;
   // bf16 token rows of the whole tile in LDS; chunk c (16 bytes) of row r sits
   // at c ^ e_swz(r), within its head.
 #pragma unroll
@@ -112,87 +109,7 @@ __device__ __forceinline__ void finish_tile(const ProjArgs& a, uint16_t* lds,
   __syncthreads();
   // Each wave takes whole rows of one head: a token half of one of two heads,
   // or a token quarter of a single one.
-  constexpr int kHeads = kChannels / kHead, kRows = kTokens * kHeads / kWaves;
-  const int nh = kHeads == 2 ? wave >> 1 : 0;
-  const int row0 = kRows * (kHeads == 2 ? wave & 1 : wave);
-  const int part = kOut ? 0 : n0 / inner;
-  const int head = kOut ? 0 : (n0 - part * inner) / kHead + nh;
-  uint16_t* out = part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
-  const bool norm = !kPlain && !kOut && part < 2;
-  constexpr bool kFull = kHl == 8;
-  constexpr int kHalf = 8 * kHl;
-  const int j = lane & 7, rg = lane >> 3;
-  const bool pair_lane = kFull || j < kHl;
-  const int chunk_a = pair_lane ? j : 2 * kHl + 2 * (j - kHl);
-  const int chunk_b = pair_lane ? j + kHl : chunk_a + 1;
-  float gam[16];
-  if (norm) {
-    const uint16_t* gsrc = part == 0 ? a.q_gamma : a.k_gamma;
-    unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_a), gam);
-    unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_b), gam + 8);
-  }
-  // Row r of the tile: this lane's two chunks, normalised and rotated.
-  auto finish_row = [&](int r, auto whole, auto rotated) __attribute__((always_inline)) {
-    const int m = m0 + r;
-    const bool valid = decltype(whole)::value || m < a.seq_len;
-    const uint16_t* row = lds + r * kChannels + nh * kHead;
-    u32x4 oa = *reinterpret_cast<const u32x4*>(row + ((chunk_a ^ e_swz(r & 15)) * 8));
-    u32x4 ob = *reinterpret_cast<const u32x4*>(row + ((chunk_b ^ e_swz(r & 15)) * 8));
-    if constexpr (decltype(rotated)::value) {
-      RopeEntry tab[8];
-      const int64_t entry = (int64_t)(decltype(whole)::value ? m : min(m, a.seq_len - 1)) * kHalf +
-                            (pair_lane ? 8 * j : 0);
-      if (kMode == H3HIP_ROUND_REFERENCE) {
-        const u32x4* tp =
-            reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.table) + entry * 4);
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const u32x4 tv = tp[q];   // (c, -s, s, c) bf16 of pairs 2q, 2q + 1
-          tab[2 * q] = RopeEntry{bf16_lo(tv[0]), bf16_lo(tv[1])};
-          tab[2 * q + 1] = RopeEntry{bf16_lo(tv[2]), bf16_lo(tv[3])};
-        }
-      } else {
-        const f32x4* tp = reinterpret_cast<const f32x4*>(a.table) + entry;
-#pragma unroll
-        for (int e = 0; e < 8; e++) tab[e] = RopeEntry{tp[e][0], tp[e][2]};
-      }
-      float xr[16];
-      unpack8(oa, xr);
-      unpack8(ob, xr + 8);
-      norm_rope<kMode, kFull>(xr, gam, pair_lane, tab, a.eps, oa, ob);
-    }
-    if (!valid) oa = ob = u32x4{0u, 0u, 0u, 0u};
-    uint16_t* dst = kOut ? a.q_out + (int64_t)m * a.ldo + n0 + nh * kHead
-                         : out + ((int64_t)head * a.seq_pad + m) * kHead;
-    if (!kOut || valid) {
-      *reinterpret_cast<u32x4*>(dst + 8 * chunk_a) = oa;
-      *reinterpret_cast<u32x4*>(dst + 8 * chunk_b) = ob;
-    }
-  };
-  // Passes of 8 rows; head-major rows end at seq_pad, a multiple of 8.
-  const int passes = kOut ? kRows / 8 : min(kRows, max(a.seq_pad - m0 - row0, 0)) / 8;
-  auto finish_rows = [&](auto whole, auto rotated) __attribute__((always_inline)) {
-    if constexpr (decltype(whole)::value) {
-#pragma unroll 2
-      for (int pass = 0; pass < kRows / 8; pass++) finish_row(row0 + 8 * pass + rg, whole, rotated);
-    } else {
-      for (int pass = 0; pass < passes; pass++) finish_row(row0 + 8 * pass + rg, whole, rotated);
-    }
-  };
-  const bool whole = m0 + row0 + kRows <= a.seq_len;
-  if constexpr (!kPlain && !kOut) {
-    if (norm) {
-      if (whole)
-        finish_rows(std::true_type{}, std::true_type{});
-      else
-        finish_rows(std::false_type{}, std::true_type{});
-      return;
-    }
-  }
-  if (whole)
-    finish_rows(std::true_type{}, std::false_type{});
-  else
-    finish_rows(std::false_type{}, std::false_type{});
+  finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut>(a, lds, wave, lane, m0, n0);
 }
 
 template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>

@@ -1,0 +1,23 @@
+// Arguments of the int8 projections' kernels (proj_i8.hip, proj_i8_gemm.hip).
+#pragma once
+
+#include "proj.h"
+
+namespace h3hip {
+
+// out holds what the epilogue shares with the bf16 projections (outputs, gammas,
+// table, sizes; its operands are unused). Operand rows are int8, strides in bytes.
+struct ProjI8Args {
+  ProjArgs out;
+  const int8_t* __restrict__ x;         // [seq_len, in], row stride ldx
+  const int8_t* __restrict__ w;         // [n_total, in], row stride ldw
+  const float* __restrict__ x_scale;    // [seq_len]
+  const float* __restrict__ w_scale;    // [n_total]
+  int64_t ldx, ldw;
+  int32_t in, n_total;
+  int32_t wide;   // token-major output: rows and row stride allow 16-byte stores
+};
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+}  // namespace h3hip

@@ -256,6 +256,137 @@ def out_proj(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None):
     return out
 
 
+# ------------------------------------------------------------- int8 projections
+
+def _require_same_device(t: torch.Tensor, **others):
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{name} must be on {t.device}, got {o.device}")
+
+
+def quant_rows(x: torch.Tensor, out=None):
+    """Rows of bf16 rounded to int8 with one scale a row.
+
+    x: [S, K] bf16 (row stride free, unit column stride). Returns (q, scale): int8
+    [S, K padded to a multiple of 128] (zeros past K) and fp32 [S], x being about
+    q * scale: the activations of an int8 projection, or its weights, rounded once.
+    A row holding an infinity or a NaN gets the scale NaN. ``out`` is such a pair to
+    write into."""
+    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError(f"x must be [S, K > 0] with unit column stride, got shape "
+                         f"{tuple(x.shape)} strides {x.stride()}")
+    S, K = x.shape
+    shape = (S, (K + 127) // 128 * 128)
+    _require_gpu_bf16("x", x)
+    if out is None:
+        q = torch.empty(shape, dtype=torch.int8, device=x.device)
+        scale = torch.empty((S,), dtype=torch.float32, device=x.device)
+    else:
+        q, scale = out
+        if q.shape != shape or q.dtype != torch.int8 or q.stride(1) != 1:
+            raise ValueError(f"out[0] must be int8 {shape} with unit column stride")
+        if scale.shape != (S,) or scale.dtype != torch.float32 or not scale.is_contiguous():
+            raise ValueError(f"out[1] must be contiguous fp32 [{S}]")
+        _require_same_device(x, q=q, scale=scale)
+    ldx = max(x.stride(0), K) if S <= 1 else x.stride(0)
+    ldq = max(q.stride(0), shape[1]) if S <= 1 else q.stride(0)
+    with torch.cuda.device(x.device):
+        L.check(L.lib().h3hip_quant_rows(_ptr(x), ldx, S, K, _ptr(q), ldq, _ptr(scale), _stream(x)))
+    return q, scale
+
+
+def _int8_operands(x, x_scale, w, w_scale):
+    """Checks the operands of an int8 projection; returns (rows, in, out, ldx, ldw)."""
+    for name, t in (("x", x), ("w", w)):
+        if t.dim() != 2 or t.stride(1) != 1:
+            raise ValueError(f"{name} must be 2-D with unit column stride")
+        if t.dtype != torch.int8:
+            raise ValueError(f"{name} must be int8 (quant_rows()), got {t.dtype}")
+    S, K = x.shape
+    if w.shape[1] != K:
+        raise ValueError(f"w must be [out, {K}], got {tuple(w.shape)}")
+    for name, t, n in (("x_scale", x_scale, S), ("w_scale", w_scale, w.shape[0])):
+        if t.shape != (n,) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous fp32 [{n}]")
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor (no host fallback exists)")
+    _require_same_device(x, x_scale=x_scale, w=w, w_scale=w_scale)
+    return S, K, w.shape[0], max(x.stride(0), K) if S <= 1 else x.stride(0), \
+        max(w.stride(0), K) if w.shape[0] <= 1 else w.stride(0)
+
+
+def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+            out: torch.Tensor | None = None):
+    """A projection on int8 operands: y = (x . w^T) * x_scale[:, None] * w_scale.
+
+    x: [S, K] int8 and x_scale: [S] fp32, w: [N, K] int8 and w_scale: [N] fp32, as
+    quant_rows() makes them (K a multiple of 128). Returns y [S, N] bf16 (or writes
+    ``out``, any row stride), or None when declined."""
+    S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
+    if out is None:
+        out = torch.empty((S, N), dtype=torch.bfloat16, device=x.device)
+    elif (out.dim() != 2 or out.shape != (S, N) or (out.stride(1) != 1 and N > 1)
+          or out.dtype != torch.bfloat16 or not out.is_cuda):
+        raise ValueError(f"out must be a bf16 GPU [{S}, {N}] view with unit column stride")
+    _require_same_device(x, out=out)
+    ldy = max(out.stride(0), N) if S <= 1 else out.stride(0)
+    with torch.cuda.device(x.device):
+        rc = L.lib().h3hip_proj_i8(_ptr(x), ldx, _ptr(x_scale), _ptr(w), ldw, _ptr(w_scale), K, N,
+                                   S, _ptr(out), ldy, _stream(x))
+    if L.check(rc, allow_declined=True) == L.DECLINED:
+        return None
+    return out
+
+
+def qkv_proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None,
+                table: torch.Tensor | None = None, *, heads: int, head_dim: int = 128,
+                eps: float = 1e-6, seq_pad: int | None = None,
+                rounding: int = L.ROUND_REFERENCE, out=None):
+    """qkv_proj() on int8 operands (x, x_scale, w, w_scale as for proj_i8(), w
+    [3*heads*head_dim, hidden]): the QKV product with the Q/K norm + RoPE in its
+    epilogue. Returns (q, k, v) as [heads, seq_pad, head_dim] bf16, or None when the
+    geometry is declined."""
+    S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
+    if N != 3 * heads * head_dim:
+        raise ValueError(f"w must be [{3 * heads * head_dim}, {K}], got {tuple(w.shape)}")
+    seq_pad = seq_pad or ((S + L.TILE - 1) // L.TILE) * L.TILE
+    if q_gamma is None and k_gamma is None:
+        rot = head_dim
+    else:
+        rot = _check_norm_rope(S, head_dim, q_gamma, k_gamma, table, rounding)
+        _require_same_device(x, q_gamma=q_gamma, k_gamma=k_gamma, table=table)
+    shape = (heads, seq_pad, head_dim)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=torch.bfloat16, device=x.device) for _ in range(3))
+    else:
+        for t in out:
+            _require_out(t, shape, x.device)
+    q_out, k_out, v_out = out
+    with torch.cuda.device(x.device):
+        rc = L.lib().h3hip_qkv_proj_i8(_ptr(x), ldx, _ptr(x_scale), _ptr(w), ldw, _ptr(w_scale), K,
+                                       _ptr(q_gamma), _ptr(k_gamma), eps, _ptr(table), rot,
+                                       rounding, S, seq_pad, heads, head_dim, _ptr(q_out),
+                                       _ptr(k_out), _ptr(v_out), _stream(x))
+    if L.check(rc, allow_declined=True) == L.DECLINED:
+        return None
+    return q_out, k_out, v_out
+
+
+def _check_norm_rope(S, head_dim, q_gamma, k_gamma, table, rounding) -> int:
+    """Checks what the Q/K norm and rotation read; returns rot."""
+    for name, t in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
+        if t is None or t.shape != (head_dim,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [{head_dim}]")
+        _require_gpu_bf16(name, t)
+    dt = torch.bfloat16 if rounding == L.ROUND_REFERENCE else torch.float32
+    if (table is None or not table.is_cuda or table.dtype != dt or not table.is_contiguous()
+            or table.dim() != 4 or table.shape[0] < S or table.shape[2:] != (2, 2)):
+        raise ValueError(f"table must be a contiguous {dt} [>= {S}, rot/2, 2, 2] GPU tensor "
+                         "(rope_table() with the same rounding mode)")
+    return 2 * table.shape[1]
+
+
 # -------------------------------------------------------------------- attention
 
 def _head_major_qkv(plan: TilePlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
