@@ -56,9 +56,15 @@ SGPRS = list(range(64, 77))
 
 
 class Gen:
+    """One tile shape's loop. The int8 loops (gen_gemm_i8_loop.py) are the same stream
+    with another product: a row's 128 bytes a step are then 128 values."""
+    VARIANTS = VARIANTS
+    MFMA = "v_mfma_f32_16x16x32_bf16"
+    LABEL = "L_gemm"
+
     def __init__(self, name):
         self.name = name
-        self.na, self.mb, self.rw, self.rx = VARIANTS[name]
+        self.na, self.mb, self.rw, self.rx = self.VARIANTS[name]
         self.w_slot, self.x_slot = 32 * self.na * ROW, 32 * self.mb * ROW
         self.x_at = self.rw * self.w_slot            # x ring after the W ring
         self.lds = self.x_at + self.rx * self.x_slot
@@ -146,7 +152,7 @@ class Gen:
         for k in range(n):
             na, mb = divmod(k, self.mb)
             c = self.C(na, mb)
-            self.emit(f"v_mfma_f32_16x16x32_bf16 {c}, {self.A(u, na)}, {self.B(u, mb)}, {c}")
+            self.emit(f"{self.MFMA} {c}, {self.A(u, na)}, {self.B(u, mb)}, {c}")
             # the reads over the first three quarters, so that they are back
             want = min(nr, -(-(k + 1) * nr * 4 // (3 * n)))
             while done_r < want:
@@ -179,7 +185,7 @@ class Gen:
 
     def generate(self):
         em = self.emit
-        end, loop = f"L_gemm{self.name}_end_%=", f"L_gemm{self.name}_loop_%="
+        end, loop = f"{self.LABEL}{self.name}_end_%=", f"{self.LABEL}{self.name}_loop_%="
         em(f"s_mov_b32 {SM0}, m0")
         for i, r in enumerate(("x_lo", "x_hi", "x_rec")):
             em(f"s_mov_b32 s{64 + i}, %[{r}]")
@@ -214,7 +220,7 @@ class Gen:
         waits = [self.step(t, t, end) for t in range(self.unroll)]
         em(f"s_branch {loop}", f"{end}:")
         # The waits of the unrolled steps hold for every later round too.
-        later = Gen(self.name)
+        later = type(self)(self.name)
         later.issued = list(self.issued)
         assert [later.step(t, self.unroll + t, end) for t in range(self.unroll)] == waits
         assert max(waits) < 64
@@ -227,11 +233,11 @@ class Gen:
         return regs + ["scc", "memory"]
 
 
-def render():
-    out = ["// Generated by gen_gemm_loop.py -- do not edit; regenerate instead.",
-           f"#define H3_GEMM_WAVES {WAVES}"]
-    for name, (na, mb, rw, rx) in VARIANTS.items():
-        g = Gen(name)
+def render(gen=Gen, script="gen_gemm_loop.py", macro="H3_GEMM"):
+    out = [f"// Generated by {script} -- do not edit; regenerate instead.",
+           f"#define {macro}_WAVES {WAVES}"]
+    for name, (na, mb, rw, rx) in gen.VARIANTS.items():
+        g = gen(name)
         lines = g.generate()
         body = " \\\n".join('  "' + ln + '\\n"' for ln in lines)
         ins = [f'"{{v{at + i}}}"({arg}[{i}])'
@@ -240,12 +246,12 @@ def render():
                for i in range(n)]
         acc = [f'"=&{{a[{32 * i}:{32 * i + 31}]}}"(C[{i}])' for i in range(-(-na * mb // 8))]
         out += [f"// {32 * na} channels x {32 * mb} tokens: {len(lines)} lines.",
-                f"#define H3_GEMM_LDS_{name} {g.lds}",
-                f"#define H3_GEMM_BASES_{name} {g.bases}",
-                f"#define H3_GEMM_LOOP_{name} \\\n" + body + "\n",
-                f"#define H3_GEMM_OUT_{name}(C) " + ", ".join(acc),
-                f"#define H3_GEMM_IN_{name}(RA, RB, XV, WV) " + ", ".join(ins),
-                f"#define H3_GEMM_CLOBBERS_{name} " + ", ".join(f'"{r}"' for r in g.clobbers())]
+                f"#define {macro}_LDS_{name} {g.lds}",
+                f"#define {macro}_BASES_{name} {g.bases}",
+                f"#define {macro}_LOOP_{name} \\\n" + body + "\n",
+                f"#define {macro}_OUT_{name}(C) " + ", ".join(acc),
+                f"#define {macro}_IN_{name}(RA, RB, XV, WV) " + ", ".join(ins),
+                f"#define {macro}_CLOBBERS_{name} " + ", ".join(f'"{r}"' for r in g.clobbers())]
     return "\n".join(out) + "\n"
 
 

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "proj.h"
+#include "proj_i8_tile.h"
 
 namespace h3hip {
 
@@ -19,5 +20,9 @@ struct ProjI8Args {
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Launches proj_i8_gemm_kernel on one of its tile shapes (proj_i8_gemm.hip).
+int launch_proj_i8_gemm(const ProjI8Args& a, ProjI8Tile tile, int32_t rounding, bool plain, bool out,
+                        hipStream_t stream);
 
 }  // namespace h3hip

@@ -16,9 +16,7 @@
 // order of k within a step is free as long as both operands share it: lane (g, lr)
 // takes bytes 32 g .. 32 g + 31 of row lr for the step's two products, so that a row's
 // 128-byte line is read by one instruction pair.
-#include <algorithm>
 #include <climits>
-#include <cmath>
 
 #include "proj_i8.h"
 #include "proj_rows.h"
@@ -30,6 +28,7 @@ namespace {
 constexpr int kHeadDim = 128;
 constexpr int kStepBytes = 128;
 constexpr int kRowTokens = 16;   // tokens of a workgroup
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;   // a launch has fewer
 
 // kBlocks blocks of 16 channels a workgroup, kSplit waves for each.
 template <int kBlocks, int kSplit>
@@ -115,6 +114,10 @@ __global__ __launch_bounds__(512 * kSplit) void qkv_proj_i8_rows_kernel(ProjI8Ar
   const int heads3 = 3 * a.out.heads;
   const int m0 = (int)(blockIdx.x / heads3) * kRowTokens;
   const int n0 = (int)(blockIdx.x % heads3) * kHeadDim;
+  if (m0 >= a.out.seq_len) {
+    zero_tile_rows<kRowTokens, kHeadDim, 512 * kSplit>(a.out, threadIdx.x, m0, n0);
+    return;
+  }
   const i32x4 acc = few_rows_sum<kBlocks, kSplit>(a, n0, m0, wave, lane, part);
   if (wave < kBlocks) {
     const f32x4 w4 = *reinterpret_cast<const f32x4*>(a.w_scale + n0 + 16 * wave + 4 * g);
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(512 * kSplit) void qkv_proj_i8_rows_kernel(ProjI8Ar
 template <int kSplit>
 int launch_qkv_rows(const ProjI8Args& a, int32_t rounding, bool plain, hipStream_t st) {
   const int64_t tiles = (int64_t)(a.out.seq_pad / kRowTokens) * 3 * a.out.heads;
-  H3_REQUIRE(tiles * 512 * kSplit < ((int64_t)1 << 32), H3HIP_EINVAL,
+  H3_REQUIRE(tiles * 512 * kSplit < kMaxThreads, H3HIP_EINVAL,
              "too many rows x heads for one launch (%lld tiles)", (long long)tiles);
   const dim3 grid((unsigned)tiles), block(512 * kSplit);
   constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32;
@@ -210,20 +213,15 @@ extern "C" int h3hip_proj_i8(const void* x, int64_t ldx, const float* x_scale, c
   a.in = in_features;
   a.n_total = out_features;
   a.wide = ldy % 8 == 0 && aligned(y, 16);
+  const ProjI8Tile tile = pick_proj_i8_tile(rows, rows, out_features, false);
+  if (tile != ProjI8Tile::kRows)
+    return launch_proj_i8_gemm(a, tile, H3HIP_ROUND_REFERENCE, true, true, as_stream(stream));
   constexpr int kSplit = 8;
-  // A launch takes fewer than 2^32 threads: row ranges that fit, one after another.
-  const int64_t tiles_n = ((int64_t)out_features + 15) / 16;
-  const int64_t most = (((int64_t)1 << 32) - 1) / (64 * kSplit) / tiles_n;
-  H3_REQUIRE(most > 0, H3HIP_EINVAL, "too many channels (%d)", out_features);
-  for (int64_t m = 0; m < rows; m += most * kRowTokens) {
-    ProjI8Args c = a;
-    c.out.seq_len = (int32_t)std::min((int64_t)rows - m, most * kRowTokens);
-    c.x += m * ldx;
-    c.x_scale += m;
-    c.out.q_out += m * ldy;
-    const int64_t tiles = (c.out.seq_len + kRowTokens - 1) / kRowTokens * tiles_n;
-    proj_i8_rows_kernel<kSplit><<<dim3((unsigned)tiles), 64 * kSplit, 0, as_stream(stream)>>>(c);
-  }
+  const int64_t tiles = (((int64_t)rows + kRowTokens - 1) / kRowTokens) *
+                        (((int64_t)out_features + 15) / 16);
+  H3_REQUIRE(tiles * 64 * kSplit < kMaxThreads, H3HIP_EINVAL,
+             "too many rows x channels for one launch (%d x %d)", rows, out_features);
+  proj_i8_rows_kernel<kSplit><<<dim3((unsigned)tiles), 64 * kSplit, 0, as_stream(stream)>>>(a);
   return check_launch("proj_i8_rows_kernel");
 }
 
@@ -277,5 +275,8 @@ extern "C" int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scal
   a.ldw = ldw;
   a.in = hidden;
   a.n_total = 3 * heads * kHeadDim;
+  const ProjI8Tile tile = pick_proj_i8_tile(seq_len, seq_pad, a.n_total, true);
+  if (tile != ProjI8Tile::kRows)
+    return launch_proj_i8_gemm(a, tile, rounding, plain, false, as_stream(stream));
   return launch_qkv_rows<2>(a, rounding, plain, as_stream(stream));
 }

@@ -1,0 +1,211 @@
+// The int8 projections' GEMM on four waves: tiles of W x^T for any number of rows
+// beyond the few that proj_i8.hip takes.
+//
+// The loop is the bf16 GEMM's (proj_gemm.hip has its layout and why it is four waves)
+// with v_mfma_i32_16x16x64_i8 in place of the bf16 product: twice the operations for the
+// same LDS bytes, loads and matrix-core cycles (gen_gemm_i8_loop.py). The 256 accumulators
+// are int32 and exact. Rows of x past seq_len and of W past its last read as zeros, so
+// a tile at either edge needs no case of its own before its stores.
+//
+// Epilogue: each sum to fp32, times its token's and its channel's scale, to bf16, into
+// LDS as token rows, and from there what the bf16 projections do (proj_rows.h).
+#include "gemm_i8_loop.inc"
+#include "proj_i8.h"
+#include "proj_rows.h"
+#include "tile_order.h"
+
+namespace h3hip {
+
+namespace {
+
+constexpr int kWaves = H3_GEMM_I8_WAVES;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kStep = 128;               // reduction per step (bytes)
+
+typedef int i32x32 __attribute__((ext_vector_type(32)));
+// A wave's accumulators, 8 blocks of 16 x 16 to a vector (the last may be part used).
+template <int kNA, int kMB>
+constexpr int kAccs = (kNA * kMB + 7) / 8;
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
+#define H3_SCALARS                                                                          \
+  [x_lo] "s"(x_lo), [x_hi] "s"(x_hi), [x_rec] "s"(x_rec), [w_lo] "s"(w_lo), [w_hi] "s"(w_hi), \
+      [w_rec] "s"(w_rec), [steps] "s"(steps), [m0x] "s"(m0x), [m0w] "s"(m0w)
+
+// One tile shape: its LDS and its reduction loop, from lane offsets and scalars
+// to accumulators.
+template <int kNA, int kMB>
+struct Shape;
+#define H3_SHAPE(NA, MB, NAME)                                                               \
+  template <>                                                                                \
+  struct Shape<NA, MB> {                                                                     \
+    static constexpr int kLds = H3_GEMM_I8_LDS_##NAME, kBases = H3_GEMM_I8_BASES_##NAME;       \
+    static __device__ __forceinline__ void reduce(i32x32 (&c)[kAccs<NA, MB>], const int* ra,   \
+                                                  const int* rb, const int* xv, const int* wv, \
+                                                  uint32_t x_lo, uint32_t x_hi, uint32_t x_rec, \
+                                                  uint32_t w_lo, uint32_t w_hi, uint32_t w_rec, \
+                                                  uint32_t steps, uint32_t m0x, uint32_t m0w) { \
+      asm volatile(H3_GEMM_I8_LOOP_##NAME                                                    \
+                   : H3_GEMM_I8_OUT_##NAME(c)                                                \
+                   : H3_GEMM_I8_IN_##NAME(ra, rb, xv, wv), H3_SCALARS                        \
+                   : H3_GEMM_I8_CLOBBERS_##NAME);                                            \
+    }                                                                                        \
+  };
+H3_SHAPE(8, 8, 256x256)
+H3_SHAPE(8, 7, 256x224)
+H3_SHAPE(8, 6, 256x192)
+H3_SHAPE(8, 5, 256x160)
+H3_SHAPE(8, 4, 256x128)
+H3_SHAPE(4, 6, 128x192)
+H3_SHAPE(4, 5, 128x160)
+H3_SHAPE(4, 4, 128x128)
+H3_SHAPE(4, 2, 128x64)
+
+// Scales of channels n .. n + 3.
+__device__ __forceinline__ f32x4 channel_scales(const ProjI8Args& a, int64_t n, bool whole) {
+  if (whole || n + 4 <= a.n_total) return *reinterpret_cast<const f32x4*>(a.w_scale + n);
+  f32x4 s;
+#pragma unroll
+  for (int i = 0; i < 4; i++) s[i] = a.w_scale[min(n + i, (int64_t)a.n_total - 1)];
+  return s;
+}
+
+// The tile's epilogue. Accumulator (na, mb) of lane (g, lr): channels
+// 16 (kNA wc + na) + 4g .. +3 of token 16 (kMB wt + mb) + lr.
+template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>
+__device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
+                                            const i32x32 (&c)[kAccs<kNA, kMB>], int wave, int lane,
+                                            int m0, int n0) {
+  constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
+  const int wc = wave >> 1, wt = wave & 1, lr = lane & 15, g = lane >> 4;
+  float xs[kMB];
+#pragma unroll
+  for (int mb = 0; mb < kMB; mb++)
+    xs[mb] = a.x_scale[min(m0 + 16 * (kMB * wt + mb) + lr, a.out.seq_len - 1)];
+  // bf16 token rows of the whole tile in LDS; chunk c (16 bytes) of row r sits
+  // at c ^ e_swz(r), within its head.
+#pragma unroll
+  for (int na = 0; na < kNA; na++) {
+    const f32x4 ws = channel_scales(a, n0 + 16 * (kNA * wc + na) + 4 * g, !kOut);
+    const int chunk = 2 * (kNA * wc + na) + (g >> 1);
+    const int pos = (chunk & 16) | ((chunk & 15) ^ e_swz(lr));
+#pragma unroll
+    for (int mb = 0; mb < kMB; mb++) {
+      const int r = 16 * (kMB * wt + mb) + lr, e = 4 * (kMB * na + mb);
+      const i32x32& v = c[e / 32];
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = (float)v[e % 32 + i] * xs[mb] * ws[i];
+      *reinterpret_cast<u32x2*>(lds + r * kChannels + pos * 8 + 4 * (g & 1)) =
+          u32x2{cvt_pk(y[0], y[1]), cvt_pk(y[2], y[3])};
+    }
+  }
+  __syncthreads();
+  finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, kOut>(
+      a.out, lds, wave, lane, m0, n0, a.wide != 0);
+}
+
+template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>
+__global__ __launch_bounds__(kThreads, 1) void proj_i8_gemm_kernel(ProjI8Args a) {
+  using S = Shape<kNA, kMB>;
+  constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
+  static_assert(S::kLds >= 2 * kTokens * kChannels, "the epilogue's rows fit in the rings");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds / 2];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wc = wave >> 1, wt = wave & 1;   // channel and token half of the tile
+  const TileOrder order{a.out.tiles_m, (a.n_total + kChannels - 1) / kChannels, a.out.chunk};
+  const int xcd = blockIdx.x % kOrderXcds, slot = blockIdx.x / kOrderXcds;
+  if (slot >= order.length(xcd)) return;
+  const uint32_t tile = order.tile(xcd, slot);
+  const int m0 = (int)(tile >> 16) * kTokens, n0 = (int)(tile & 0xffff) * kChannels;
+  if (!kOut && m0 >= a.out.seq_len) {
+    zero_tile_rows<kTokens, kChannels, kThreads>(a.out, threadIdx.x, m0, n0);
+    return;
+  }
+
+  const int lr = lane & 15, g = lane >> 4;
+  const uint32_t lds_base = uniform((uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t*)lds);
+  int ra[2 * S::kBases], rb[2 * S::kBases], xv[kMB], wv[kNA];
+#pragma unroll
+  for (int b = 0; b < S::kBases; b++)
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int at = (int)lds_base + 65536 * b + (((4 * u + g) ^ p_swz(lr)) * 16);
+      ra[2 * b + u] = at + (16 * kNA * wc + lr) * 128;
+      rb[2 * b + u] = at + (16 * kMB * wt + lr) * 128;
+    }
+  const int ldx = (int)a.ldx, ldw = (int)a.ldw;
+  auto load_offset = [&](int rows, int i, int ld) __attribute__((always_inline)) {
+    const int r = rows * wave + 8 * i + (lane >> 3);
+    return r * ld + (((lane & 7) ^ p_swz(r)) * 16) - 1024 * (i & 3);
+  };
+#pragma unroll
+  for (int i = 0; i < kMB; i++) xv[i] = load_offset(8 * kMB, i, ldx);
+#pragma unroll
+  for (int i = 0; i < kNA; i++) wv[i] = load_offset(8 * kNA, i, ldw);
+  const uint64_t xp = (uint64_t)(uintptr_t)(a.x + (int64_t)m0 * a.ldx);
+  const uint64_t wp = (uint64_t)(uintptr_t)(a.w + (int64_t)n0 * a.ldw);
+  const uint32_t x_lo = uniform((uint32_t)xp), x_hi = uniform((uint32_t)(xp >> 32));
+  const uint32_t w_lo = uniform((uint32_t)wp), w_hi = uniform((uint32_t)(wp >> 32));
+  // Bytes of the tile's rows that exist: what lies past them reads as zero.
+  const int x_rows = min(a.out.seq_len - m0, kTokens), w_rows = min(a.n_total - n0, kChannels);
+  const uint32_t x_rec = uniform((uint32_t)((x_rows - 1) * ldx + a.in));
+  const uint32_t w_rec = uniform((uint32_t)((w_rows - 1) * ldw + a.in));
+  const uint32_t steps = uniform((uint32_t)(a.in / kStep));
+  const uint32_t m0w = uniform(lds_base + 1024u * kNA * wave);
+  const uint32_t m0x = uniform(lds_base + 1024u * kMB * wave);
+  i32x32 c[kAccs<kNA, kMB>];
+  S::reduce(c, ra, rb, xv, wv, x_lo, x_hi, x_rec, w_lo, w_hi, w_rec, steps, m0x, m0w);
+
+  // The lane again, from the lane counter: kept from before the loop it would
+  // be spilled across it.
+  int lane2;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane2));
+  finish_tile<kNA, kMB, kMode, kHl, kPlain, kOut>(a, lds, c, wave, lane2, m0, n0);
+}
+
+template <int kNA, int kMB>
+int launch(ProjI8Args a, int32_t rounding, bool plain, bool out, hipStream_t st) {
+  const ProjGrid g = proj_i8_grid(out ? a.out.seq_len : a.out.seq_pad, a.n_total, 32 * kMB, 32 * kNA);
+  a.out.tiles_m = g.order.tiles_m;
+  a.out.chunk = g.order.chunk;
+  const dim3 grid(kOrderXcds * g.longest);
+  constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32;
+  if (out)
+    proj_i8_gemm_kernel<kNA, kMB, kRef, 8, true, true><<<grid, kThreads, 0, st>>>(a);
+  else if (plain)
+    proj_i8_gemm_kernel<kNA, kMB, kRef, 8, true, false><<<grid, kThreads, 0, st>>>(a);
+  else if (rounding == kRef && a.out.rot == 128)
+    proj_i8_gemm_kernel<kNA, kMB, kRef, 8, false, false><<<grid, kThreads, 0, st>>>(a);
+  else if (rounding == kRef)
+    proj_i8_gemm_kernel<kNA, kMB, kRef, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+  else if (a.out.rot == 128)
+    proj_i8_gemm_kernel<kNA, kMB, kF32, 8, false, false><<<grid, kThreads, 0, st>>>(a);
+  else
+    proj_i8_gemm_kernel<kNA, kMB, kF32, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+  return check_launch("proj_i8_gemm_kernel");
+}
+
+}  // namespace
+
+int launch_proj_i8_gemm(const ProjI8Args& a, ProjI8Tile tile, int32_t rounding, bool plain, bool out,
+                        hipStream_t stream) {
+  switch (tile) {
+    case ProjI8Tile::k256x256: return launch<8, 8>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x224: return launch<8, 7>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x192: return launch<8, 6>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x160: return launch<8, 5>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x128: return launch<8, 4>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x192: return launch<4, 6>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x160: return launch<4, 5>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x128: return launch<4, 4>(a, rounding, plain, out, stream);
+    default: return launch<4, 2>(a, rounding, plain, out, stream);
+  }
+}
+
+}  // namespace h3hip

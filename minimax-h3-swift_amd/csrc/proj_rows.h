@@ -22,6 +22,21 @@ __device__ __forceinline__ void store_row_chunk(uint16_t* dst, u32x4 v, int left
     if (e < left) dst[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
 }
 
+// Zeros into rows m0 .. of the heads of channels n0 ..: a tile of padding rows only.
+template <int kTokens, int kChannels, int kThreads>
+__device__ __forceinline__ void zero_tile_rows(const ProjArgs& a, int tid, int m0, int n0) {
+  constexpr int kHead = 128, kChunks = kHead / 8;
+  const int inner = a.heads * kHead, part = n0 / inner;
+  const int head0 = (n0 - part * inner) / kHead;
+  uint16_t* out = part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
+  for (int i = tid; i < kTokens * (kChannels / 8); i += kThreads) {
+    const int head = head0 + i / (kTokens * kChunks), r = i / kChunks % kTokens;
+    if (m0 + r < a.seq_pad)
+      *reinterpret_cast<u32x4*>(out + ((int64_t)head * a.seq_pad + m0 + r) * kHead +
+                                8 * (i % kChunks)) = u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
 // Rows of kChannels in LDS, chunk c (16 bytes) of row r at c ^ e_swz(r) within its
 // head. Each of kRowWaves waves takes whole rows of one head, 8 at a time in the
 // prologue's 8-lane layout. kHl = rot / 16 (8-channel chunks per rotation half);
