@@ -258,10 +258,45 @@ def out_proj(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None):
 
 # ------------------------------------------------------------- int8 projections
 
-def _require_same_device(t: torch.Tensor, **others):
-    for name, o in others.items():
-        if o is not None and o.device != t.device:
-            raise ValueError(f"{name} must be on {t.device}, got {o.device}")
+# These calls are as short as their launches, so what they check is checked cheaply:
+# the raw stream handle without a Stream object, the device switched only where the
+# operands are not on the current one.
+
+def _run(fn, device: torch.device, *args) -> int:
+    """fn(*args, stream) on the current stream of ``device``; DECLINED or OK."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    return rc if rc == L.OK else L.check(rc, allow_declined=True)
+
+
+def _require_same_device(device: torch.device, **others):
+    for name, t in others.items():
+        if t.device != device:
+            raise ValueError(f"{name} must be on {device}, got {t.device}")
+
+
+def _rows(name: str, t: torch.Tensor, dtype) -> int:
+    """The row stride of a 2-D tensor whose rows are contiguous (of a single row, any that
+    covers it)."""
+    if t.dtype != dtype or t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D {dtype}, got {t.dim()}-D {t.dtype}")
+    ld, step = t.stride()
+    rows, cols = t.shape
+    if step != 1 and cols > 1:
+        raise ValueError(f"{name} must have unit column stride, got strides {t.stride()}")
+    return ld if rows > 1 else max(ld, cols)
+
+
+def _vector(name: str, t: torch.Tensor, n: int, device: torch.device):
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous fp32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
 
 
 def quant_rows(x: torch.Tensor, out=None):
@@ -272,47 +307,41 @@ def quant_rows(x: torch.Tensor, out=None):
     q * scale: the activations of an int8 projection, or its weights, rounded once.
     A row holding an infinity or a NaN gets the scale NaN. ``out`` is such a pair to
     write into."""
-    if x.dim() != 2 or x.shape[1] == 0 or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ValueError(f"x must be [S, K > 0] with unit column stride, got shape "
-                         f"{tuple(x.shape)} strides {x.stride()}")
+    ldx = _rows("x", x, torch.bfloat16)
     S, K = x.shape
-    shape = (S, (K + 127) // 128 * 128)
-    _require_gpu_bf16("x", x)
+    if K == 0:
+        raise ValueError("x must be [S, K > 0]")
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor (no host fallback exists)")
+    device, pad = x.device, (K + 127) // 128 * 128
     if out is None:
-        q = torch.empty(shape, dtype=torch.int8, device=x.device)
-        scale = torch.empty((S,), dtype=torch.float32, device=x.device)
+        q = torch.empty((S, pad), dtype=torch.int8, device=device)
+        scale = torch.empty(S, dtype=torch.float32, device=device)
+        ldq = pad
     else:
         q, scale = out
-        if q.shape != shape or q.dtype != torch.int8 or q.stride(1) != 1:
-            raise ValueError(f"out[0] must be int8 {shape} with unit column stride")
-        if scale.shape != (S,) or scale.dtype != torch.float32 or not scale.is_contiguous():
-            raise ValueError(f"out[1] must be contiguous fp32 [{S}]")
-        _require_same_device(x, q=q, scale=scale)
-    ldx = max(x.stride(0), K) if S <= 1 else x.stride(0)
-    ldq = max(q.stride(0), shape[1]) if S <= 1 else q.stride(0)
-    with torch.cuda.device(x.device):
-        L.check(L.lib().h3hip_quant_rows(_ptr(x), ldx, S, K, _ptr(q), ldq, _ptr(scale), _stream(x)))
+        ldq = _rows("out[0]", q, torch.int8)
+        if q.shape != (S, pad):
+            raise ValueError(f"out[0] must be [{S}, {pad}], got {tuple(q.shape)}")
+        _require_same_device(device, q=q)
+        _vector("out[1]", scale, S, device)
+    _run(L.lib().h3hip_quant_rows, device, x.data_ptr(), ldx, S, K, q.data_ptr(), ldq,
+         scale.data_ptr())
     return q, scale
 
 
 def _int8_operands(x, x_scale, w, w_scale):
-    """Checks the operands of an int8 projection; returns (rows, in, out, ldx, ldw)."""
-    for name, t in (("x", x), ("w", w)):
-        if t.dim() != 2 or t.stride(1) != 1:
-            raise ValueError(f"{name} must be 2-D with unit column stride")
-        if t.dtype != torch.int8:
-            raise ValueError(f"{name} must be int8 (quant_rows()), got {t.dtype}")
-    S, K = x.shape
-    if w.shape[1] != K:
-        raise ValueError(f"w must be [out, {K}], got {tuple(w.shape)}")
-    for name, t, n in (("x_scale", x_scale, S), ("w_scale", w_scale, w.shape[0])):
-        if t.shape != (n,) or t.dtype != torch.float32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous fp32 [{n}]")
+    """Checks the operands of an int8 projection; returns (ldx, ldw)."""
+    ldx, ldw = _rows("x", x, torch.int8), _rows("w", w, torch.int8)
+    if w.shape[1] != x.shape[1]:
+        raise ValueError(f"w must be [out, {x.shape[1]}], got {tuple(w.shape)}")
+    device = x.device
+    _require_same_device(device, w=w)
+    _vector("x_scale", x_scale, x.shape[0], device)
+    _vector("w_scale", w_scale, w.shape[0], device)
     if not x.is_cuda:
         raise ValueError("x must be a GPU tensor (no host fallback exists)")
-    _require_same_device(x, x_scale=x_scale, w=w, w_scale=w_scale)
-    return S, K, w.shape[0], max(x.stride(0), K) if S <= 1 else x.stride(0), \
-        max(w.stride(0), K) if w.shape[0] <= 1 else w.stride(0)
+    return ldx, ldw
 
 
 def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -322,20 +351,19 @@ def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     x: [S, K] int8 and x_scale: [S] fp32, w: [N, K] int8 and w_scale: [N] fp32, as
     quant_rows() makes them (K a multiple of 128). Returns y [S, N] bf16 (or writes
     ``out``, any row stride), or None when declined."""
-    S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
+    ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
+    (S, K), N = x.shape, w.shape[0]
     if out is None:
         out = torch.empty((S, N), dtype=torch.bfloat16, device=x.device)
-    elif (out.dim() != 2 or out.shape != (S, N) or (out.stride(1) != 1 and N > 1)
-          or out.dtype != torch.bfloat16 or not out.is_cuda):
-        raise ValueError(f"out must be a bf16 GPU [{S}, {N}] view with unit column stride")
-    _require_same_device(x, out=out)
-    ldy = max(out.stride(0), N) if S <= 1 else out.stride(0)
-    with torch.cuda.device(x.device):
-        rc = L.lib().h3hip_proj_i8(_ptr(x), ldx, _ptr(x_scale), _ptr(w), ldw, _ptr(w_scale), K, N,
-                                   S, _ptr(out), ldy, _stream(x))
-    if L.check(rc, allow_declined=True) == L.DECLINED:
-        return None
-    return out
+        ldy = N
+    else:
+        ldy = _rows("out", out, torch.bfloat16)
+        if out.shape != (S, N):
+            raise ValueError(f"out must be [{S}, {N}], got {tuple(out.shape)}")
+        _require_same_device(x.device, out=out)
+    rc = _run(L.lib().h3hip_proj_i8, x.device, x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(),
+              ldw, w_scale.data_ptr(), K, N, S, out.data_ptr(), ldy)
+    return None if rc == L.DECLINED else out
 
 
 def qkv_proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -347,30 +375,30 @@ def qkv_proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     [3*heads*head_dim, hidden]): the QKV product with the Q/K norm + RoPE in its
     epilogue. Returns (q, k, v) as [heads, seq_pad, head_dim] bf16, or None when the
     geometry is declined."""
-    S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
-    if N != 3 * heads * head_dim:
+    ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
+    S, K = x.shape
+    device = x.device
+    if w.shape[0] != 3 * heads * head_dim:
         raise ValueError(f"w must be [{3 * heads * head_dim}, {K}], got {tuple(w.shape)}")
-    seq_pad = seq_pad or ((S + L.TILE - 1) // L.TILE) * L.TILE
+    seq_pad = seq_pad or (S + L.TILE - 1) // L.TILE * L.TILE
     if q_gamma is None and k_gamma is None:
-        rot = head_dim
+        rot, gq, gk, tab = head_dim, None, None, None
     else:
         rot = _check_norm_rope(S, head_dim, q_gamma, k_gamma, table, rounding)
-        _require_same_device(x, q_gamma=q_gamma, k_gamma=k_gamma, table=table)
+        _require_same_device(device, q_gamma=q_gamma, k_gamma=k_gamma, table=table)
+        gq, gk, tab = q_gamma.data_ptr(), k_gamma.data_ptr(), table.data_ptr()
     shape = (heads, seq_pad, head_dim)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=torch.bfloat16, device=x.device) for _ in range(3))
+        out = tuple(torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(3))
     else:
+        out = tuple(out)
         for t in out:
-            _require_out(t, shape, x.device)
+            _require_out(t, shape, device)
     q_out, k_out, v_out = out
-    with torch.cuda.device(x.device):
-        rc = L.lib().h3hip_qkv_proj_i8(_ptr(x), ldx, _ptr(x_scale), _ptr(w), ldw, _ptr(w_scale), K,
-                                       _ptr(q_gamma), _ptr(k_gamma), eps, _ptr(table), rot,
-                                       rounding, S, seq_pad, heads, head_dim, _ptr(q_out),
-                                       _ptr(k_out), _ptr(v_out), _stream(x))
-    if L.check(rc, allow_declined=True) == L.DECLINED:
-        return None
-    return q_out, k_out, v_out
+    rc = _run(L.lib().h3hip_qkv_proj_i8, device, x.data_ptr(), ldx, x_scale.data_ptr(),
+              w.data_ptr(), ldw, w_scale.data_ptr(), K, gq, gk, eps, tab, rot, rounding, S, seq_pad,
+              heads, head_dim, q_out.data_ptr(), k_out.data_ptr(), v_out.data_ptr())
+    return None if rc == L.DECLINED else out
 
 
 def _check_norm_rope(S, head_dim, q_gamma, k_gamma, table, rounding) -> int:
