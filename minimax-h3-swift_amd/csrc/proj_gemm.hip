@@ -107,15 +107,16 @@ __device__ __forceinline__ void finish_tile(const ProjArgs& a, uint16_t* lds,
       *reinterpret_cast<u32x2*>(lds + r * kChannels + pos * 8 + 4 * (g & 1)) = v2;
     }
   __syncthreads();
-  // Each wave takes whole rows of one head: a token half of one of two heads,
-  // or a token quarter of a single one.
-  finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut>(a, lds, wave, lane, m0, n0);
+  finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut>(
+      a, lds, reinterpret_cast<RopeEntry*>(lds + kTokens * kChannels), wave, lane, m0, n0);
 }
 
 template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>
 __global__ __launch_bounds__(kThreads, 1) void proj_gemm_kernel(ProjArgs a) {
   using S = Shape<kNA, kMB>;
   constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
+  static_assert(S::kLds >= 2 * kTokens * kChannels + kWaves * kRowTableLds,
+                "the epilogue's rows and tables fit in the rings");
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds / 2];
 
   const int lane = threadIdx.x & 63;

@@ -109,6 +109,8 @@ __global__ __launch_bounds__(512 * kSplit) void qkv_proj_i8_rows_kernel(ProjI8Ar
   constexpr int kBlocks = kHeadDim / 16;
   __shared__ i32x4 part[kBlocks * kSplit][64];
   __shared__ __attribute__((aligned(16))) uint16_t rows[kRowTokens * kHeadDim];
+  constexpr int kRowWaves = kRowTokens / 8;
+  __shared__ __attribute__((aligned(16))) RopeEntry tables[kRowWaves * 512];
   const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int heads3 = 3 * a.out.heads;
@@ -128,10 +130,9 @@ __global__ __launch_bounds__(512 * kSplit) void qkv_proj_i8_rows_kernel(ProjI8Ar
         u32x2{cvt_pk(y[0], y[1]), cvt_pk(y[2], y[3])};
   }
   __syncthreads();
-  constexpr int kRowWaves = kRowTokens / 8;
   if (wave < kRowWaves)
-    finish_tile_rows<kRowTokens, kHeadDim, kRowWaves, kMode, kHl, kPlain, false>(a.out, rows, wave,
-                                                                                 lane, m0, n0);
+    finish_tile_rows<kRowTokens, kHeadDim, kRowWaves, kMode, kHl, kPlain, false>(
+        a.out, rows, tables, wave, lane, m0, n0);
 }
 
 template <int kSplit>

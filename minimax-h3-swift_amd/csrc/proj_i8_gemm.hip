@@ -105,14 +105,16 @@ __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
   }
   __syncthreads();
   finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, kOut>(
-      a.out, lds, wave, lane, m0, n0, a.wide != 0);
+      a.out, lds, reinterpret_cast<RopeEntry*>(lds + kTokens * kChannels), wave, lane, m0, n0,
+      a.wide != 0);
 }
 
 template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>
 __global__ __launch_bounds__(kThreads, 1) void proj_i8_gemm_kernel(ProjI8Args a) {
   using S = Shape<kNA, kMB>;
   constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
-  static_assert(S::kLds >= 2 * kTokens * kChannels, "the epilogue's rows fit in the rings");
+  static_assert(S::kLds >= 2 * kTokens * kChannels + kWaves * kRowTableLds,
+                "the epilogue's rows and tables fit in the rings");
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds / 2];
 
   const int lane = threadIdx.x & 63;

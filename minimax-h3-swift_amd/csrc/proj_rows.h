@@ -37,72 +37,101 @@ __device__ __forceinline__ void zero_tile_rows(const ProjArgs& a, int tid, int m
   }
 }
 
+// The rotation entries of 8 token rows, from the table to the lanes of the prologue's
+// row layout: lane j of row group rg needs entries 8j .. 8j + 7 of its row, 128 bytes
+// (fp32; 64 in bf16) from its neighbour's. Loaded like that every load of a wave touches
+// 64 lines, and the loads, not the arithmetic, took the epilogue's time: at 31,885 tokens x 40
+// heads the fp32 norm and rotation added 16.6 us to a 256 x 256 tile. So the 8 lanes load 8
+// (fp32) or 16 (bf16) consecutive entries at a time, whole lines, and trade them through 4 KiB
+// of LDS of the wave's own: 6.2 us in fp32, of which 4.8 are its instructions; 10.8 in
+// reference rounding (13.4 before), whose roundings are 1.5 times the instructions.
+//
+// Entry 8b + i of a row is at unit (i >> 1) ^ u(b) of its 64-byte block b ^ rg, with u(b) =
+// (b >> 2 & 1) | (rg & 1) << 1: 32 lanes writing one entry each, or 16 reading two, then meet
+// in every bank once.
+template <int kMode, int kHl>
+struct RowTable {
+  static constexpr bool kRef = kMode == H3HIP_ROUND_REFERENCE;
+  static constexpr int kLoads = kRef ? kHl / 2 : kHl;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  u32x4 ref[kRef ? kLoads : 1];
+  f32x2 f32[kRef ? 1 : kLoads];
+
+  __device__ __forceinline__ void load(const void* table, int64_t row, int j) {
+    constexpr int kHalf = 8 * kHl;
+    if constexpr (kRef) {
+      const uint16_t* p = static_cast<const uint16_t*>(table) + (row * kHalf + 2 * j) * 4;
+#pragma unroll
+      for (int t = 0; t < kLoads; t++) ref[t] = *reinterpret_cast<const u32x4*>(p + 64 * t);
+    } else {
+      const float* p = static_cast<const float*>(table) + (row * kHalf + j) * 4 + 2;
+#pragma unroll
+      for (int t = 0; t < kLoads; t++) f32[t] = *reinterpret_cast<const f32x2*>(p + 32 * t);
+    }
+  }
+  static __device__ __forceinline__ int unit(int b, int rg) { return ((b >> 2) & 1) | (rg & 1) << 1; }
+  // From the loaded registers to tab, through the wave's lds; the pairs of pair lanes.
+  __device__ __forceinline__ void trade(RopeEntry* lds, int j, int rg, RopeEntry (&tab)[8]) {
+    RopeEntry* mine = lds + 64 * rg;
+#pragma unroll
+    for (int t = 0; t < kLoads; t++) {
+      if constexpr (kRef) {   // entries 16t + 2j, + 1; words 1 and 3 are (s, c)
+        const int b = 2 * t + (j >> 2);
+        const f32x4 v = {bf16_hi(ref[t][1]), bf16_lo(ref[t][1]), bf16_hi(ref[t][3]),
+                         bf16_lo(ref[t][3])};
+        *reinterpret_cast<f32x4*>(mine + 8 * (b ^ rg) + 2 * ((j & 3) ^ unit(b, rg))) = v;
+      } else {                // entry 8t + j, (s, c)
+        const f32x2 v = {f32[t][1], f32[t][0]};
+        *reinterpret_cast<f32x2*>(mine + 8 * (t ^ rg) + 2 * ((j >> 1) ^ unit(t, rg)) + (j & 1)) = v;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(mine + 8 * (j ^ rg) + 2 * (q ^ unit(j, rg)));
+      tab[2 * q] = RopeEntry{v[0], v[1]};
+      tab[2 * q + 1] = RopeEntry{v[2], v[3]};
+    }
+  }
+};
+constexpr int kRowTableLds = 8 * 64 * sizeof(RopeEntry);   // bytes of a wave
+
 // Rows of kChannels in LDS, chunk c (16 bytes) of row r at c ^ e_swz(r) within its
-// head. Each of kRowWaves waves takes whole rows of one head, 8 at a time in the
-// prologue's 8-lane layout. kHl = rot / 16 (8-channel chunks per rotation half);
+// head, to the outputs. Each of kRowWaves waves takes whole rows, 8 at a time in the
+// prologue's 8-lane layout, head after head, so that a row's rotation entries are
+// fetched once. kHl = rot / 16 (8-channel chunks per rotation half);
 // kPlain: every part unchanged; kOut: token-major with row stride ldo; kRagged (with
 // kOut): any output width and row stride, wide saying that the row stride and the
-// output's address allow 16-byte stores.
+// output's address allow 16-byte stores. tables: kRowTableLds bytes for each wave.
 template <int kTokens, int kChannels, int kRowWaves, int kMode, int kHl, bool kPlain, bool kOut,
           bool kRagged = false>
-__device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16_t* lds, int wave,
-                                                 int lane, int m0, int n0, bool wide = true) {
+__device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16_t* lds,
+                                                 RopeEntry* tables, int wave, int lane, int m0,
+                                                 int n0, bool wide = true) {
   constexpr int kHead = 128;
-  constexpr int kHeads = kChannels / kHead, kRows = kTokens * kHeads / kRowWaves;
-  static_assert(kRows % 8 == 0 && (kHeads == 1 || (kHeads == 2 && kRowWaves == 4)),
-                "whole passes of one head a wave");
-  const int nh = kHeads == 2 ? wave >> 1 : 0;
-  const int row0 = kRows * (kHeads == 2 ? wave & 1 : wave);
+  constexpr int kHeads = kChannels / kHead, kRows = kTokens / kRowWaves;
+  static_assert(kRows % 8 == 0, "whole passes");
+  const int row0 = kRows * wave;
   const int inner = a.heads * kHead;
   const int part = kOut ? 0 : n0 / inner;
-  const int head = kOut ? 0 : (n0 - part * inner) / kHead + nh;
+  const int head0 = kOut ? 0 : (n0 - part * inner) / kHead;
   uint16_t* out = part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
   const bool norm = !kPlain && !kOut && part < 2;
   constexpr bool kFull = kHl == 8;
-  constexpr int kHalf = 8 * kHl;
   const int j = lane & 7, rg = lane >> 3;
   const bool pair_lane = kFull || j < kHl;
   const int chunk_a = pair_lane ? j : 2 * kHl + 2 * (j - kHl);
   const int chunk_b = pair_lane ? j + kHl : chunk_a + 1;
-  float gam[16];
-  if (norm) {
-    const uint16_t* gsrc = part == 0 ? a.q_gamma : a.k_gamma;
-    unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_a), gam);
-    unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_b), gam + 8);
-  }
-  // Row r of the tile: this lane's two chunks, normalised and rotated.
-  auto finish_row = [&](int r, auto whole, auto rotated) __attribute__((always_inline)) {
-    const int m = m0 + r;
-    const bool valid = decltype(whole)::value || m < a.seq_len;
+  // This lane's two chunks of row r of the tile and head nh.
+  auto load_row = [&](int r, int nh, u32x4& oa, u32x4& ob) __attribute__((always_inline)) {
     const uint16_t* row = lds + r * kChannels + nh * kHead;
-    u32x4 oa = *reinterpret_cast<const u32x4*>(row + ((chunk_a ^ e_swz(r & 15)) * 8));
-    u32x4 ob = *reinterpret_cast<const u32x4*>(row + ((chunk_b ^ e_swz(r & 15)) * 8));
-    if constexpr (decltype(rotated)::value) {
-      RopeEntry tab[8];
-      const int64_t entry = (int64_t)(decltype(whole)::value ? m : min(m, a.seq_len - 1)) * kHalf +
-                            (pair_lane ? 8 * j : 0);
-      if (kMode == H3HIP_ROUND_REFERENCE) {
-        const u32x4* tp =
-            reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.table) + entry * 4);
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const u32x4 tv = tp[q];   // (c, -s, s, c) bf16 of pairs 2q, 2q + 1
-          tab[2 * q] = RopeEntry{bf16_lo(tv[0]), bf16_lo(tv[1])};
-          tab[2 * q + 1] = RopeEntry{bf16_lo(tv[2]), bf16_lo(tv[3])};
-        }
-      } else {
-        const f32x4* tp = reinterpret_cast<const f32x4*>(a.table) + entry;
-#pragma unroll
-        for (int e = 0; e < 8; e++) tab[e] = RopeEntry{tp[e][0], tp[e][2]};
-      }
-      float xr[16];
-      unpack8(oa, xr);
-      unpack8(ob, xr + 8);
-      norm_rope<kMode, kFull>(xr, gam, pair_lane, tab, a.eps, oa, ob);
-    }
+    oa = *reinterpret_cast<const u32x4*>(row + ((chunk_a ^ e_swz(r & 15)) * 8));
+    ob = *reinterpret_cast<const u32x4*>(row + ((chunk_b ^ e_swz(r & 15)) * 8));
+  };
+  auto store_row = [&](int r, int nh, bool valid, u32x4 oa, u32x4 ob) __attribute__((always_inline)) {
+    const int m = m0 + r;
     if (!valid) oa = ob = u32x4{0u, 0u, 0u, 0u};
     uint16_t* dst = kOut ? a.q_out + (int64_t)m * a.ldo + n0 + nh * kHead
-                         : out + ((int64_t)head * a.seq_pad + m) * kHead;
+                         : out + ((int64_t)(head0 + nh) * a.seq_pad + m) * kHead;
     if constexpr (kRagged) {
       if (valid) {
         const int left = a.n_out - n0 - nh * kHead;
@@ -116,28 +145,56 @@ __device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16
   };
   // Passes of 8 rows; head-major rows end at seq_pad, a multiple of 8.
   const int passes = kOut ? kRows / 8 : min(kRows, max(a.seq_pad - m0 - row0, 0)) / 8;
-  auto finish_rows = [&](auto whole, auto rotated) __attribute__((always_inline)) {
-    if constexpr (decltype(whole)::value) {
+  auto copy_rows = [&](int count, auto whole) __attribute__((always_inline)) {
 #pragma unroll 2
-      for (int pass = 0; pass < kRows / 8; pass++) finish_row(row0 + 8 * pass + rg, whole, rotated);
-    } else {
-      for (int pass = 0; pass < passes; pass++) finish_row(row0 + 8 * pass + rg, whole, rotated);
+    for (int pass = 0; pass < count; pass++) {
+      const int r = row0 + 8 * pass + rg;
+      const bool valid = decltype(whole)::value || m0 + r < a.seq_len;
+#pragma unroll
+      for (int nh = 0; nh < kHeads; nh++) {
+        u32x4 oa, ob;
+        load_row(r, nh, oa, ob);
+        store_row(r, nh, valid, oa, ob);
+      }
     }
   };
   const bool whole = m0 + row0 + kRows <= a.seq_len;
   if constexpr (!kPlain && !kOut) {
     if (norm) {
-      if (whole)
-        finish_rows(std::true_type{}, std::true_type{});
-      else
-        finish_rows(std::false_type{}, std::true_type{});
+      float gam[16];
+      const uint16_t* gsrc = part == 0 ? a.q_gamma : a.k_gamma;
+      unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_a), gam);
+      unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_b), gam + 8);
+      RopeEntry* mine = tables + 512 * wave;
+      RowTable<kMode, kHl> table;
+      auto fetch = [&](int pass) __attribute__((always_inline)) {
+        table.load(a.table, min(m0 + row0 + 8 * pass + rg, a.seq_len - 1), j);
+      };
+      if (passes > 0) fetch(0);
+      for (int pass = 0; pass < passes; pass++) {
+        const int r = row0 + 8 * pass + rg;
+        const bool valid = m0 + r < a.seq_len;
+        RopeEntry tab[8];
+        table.trade(mine, j, rg, tab);
+        fetch(pass + 1);   // past the last pass: a row of the table, unused
+#pragma unroll
+        for (int nh = 0; nh < kHeads; nh++) {
+          u32x4 oa, ob;
+          load_row(r, nh, oa, ob);
+          float xr[16];
+          unpack8(oa, xr);
+          unpack8(ob, xr + 8);
+          norm_rope<kMode, kFull>(xr, gam, pair_lane, tab, a.eps, oa, ob);
+          store_row(r, nh, valid, oa, ob);
+        }
+      }
       return;
     }
   }
   if (whole)
-    finish_rows(std::true_type{}, std::false_type{});
+    copy_rows(kRows / 8, std::true_type{});
   else
-    finish_rows(std::false_type{}, std::false_type{});
+    copy_rows(passes, std::false_type{});
 }
 
 }  // namespace h3hip
