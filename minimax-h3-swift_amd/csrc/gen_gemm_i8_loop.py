@@ -25,8 +25,13 @@ import gen_gemm_loop as bf16  # noqa: E402
 
 OUT = os.path.join(HERE, "gemm_i8_loop.inc")
 
-# name (channels x tokens): (NA, MB, RW, RX), as gen_gemm_loop.py's
-VARIANTS = dict(bf16.VARIANTS)
+# name (channels x tokens): (NA, MB, RW, RX). The shapes named p take at most half
+# the LDS, so that two workgroups share a CU and one's waits are the other's work.
+VARIANTS = {"256x256": (8, 8, 3, 2), "256x224": (8, 7, 3, 2), "256x192": (8, 6, 3, 2),
+            "256x160": (8, 5, 3, 3), "256x128": (8, 4, 3, 3), "128x192": (4, 6, 4, 4),
+            "128x160": (4, 5, 4, 4), "128x128": (4, 4, 5, 5),
+            "128x128p": (4, 4, 2, 2), "128x64p": (4, 2, 3, 3), "128x32p": (4, 1, 4, 4),
+            "64x64p": (2, 2, 5, 5), "32x64p": (1, 2, 6, 6), "32x32p": (1, 1, 8, 8)}
 
 
 class Gen(bf16.Gen):

@@ -1,8 +1,7 @@
-// Arguments of the int8 projections' kernels (proj_i8.hip, proj_i8_gemm.hip).
+// Arguments of the int8 projections' kernel (proj_i8_gemm.hip) and its launch.
 #pragma once
 
 #include "proj.h"
-#include "proj_i8_tile.h"
 
 namespace h3hip {
 
@@ -19,10 +18,8 @@ struct ProjI8Args {
   int32_t wide;   // token-major output: rows and row stride allow 16-byte stores
 };
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-// Launches proj_i8_gemm_kernel on one of its tile shapes (proj_i8_gemm.hip).
-int launch_proj_i8_gemm(const ProjI8Args& a, ProjI8Tile tile, int32_t rounding, bool plain, bool out,
+// Launches proj_i8_gemm_kernel on the tile shape that suits the sizes (proj_i8_gemm.hip).
+int launch_proj_i8_gemm(const ProjI8Args& a, int32_t rounding, bool plain, bool out,
                         hipStream_t stream);
 
 }  // namespace h3hip

@@ -1,4 +1,4 @@
-// The int8 projections' entry points, and the kernel for few rows.
+// The int8 projections' entry points (kernel: proj_i8_gemm.hip).
 //
 //   y[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n]
 //
@@ -9,17 +9,7 @@
 // the bf16 product normalised and rotated by the code of the bf16 path
 // (proj_rows.h), so its Q and K are h3hip_qk_norm_rope of h3hip_proj_i8's result, bit
 // for bit.
-//
-// The kernel here is v_mfma_i32_16x16x64_i8 straight from global memory: W rows as
-// the A operand, x rows as B, no LDS in the loop. A wave owns 16 channels and every
-// kSplit-th 128-byte step of the reduction; the waves' partial sums meet in LDS. The
-// order of k within a step is free as long as both operands share it: lane (g, lr)
-// takes bytes 32 g .. 32 g + 31 of row lr for the step's two products, so that a row's
-// 128-byte line is read by one instruction pair.
-#include <climits>
-
 #include "proj_i8.h"
-#include "proj_rows.h"
 
 namespace h3hip {
 
@@ -27,134 +17,6 @@ namespace {
 
 constexpr int kHeadDim = 128;
 constexpr int kStepBytes = 128;
-constexpr int kRowTokens = 16;   // tokens of a workgroup
-constexpr int64_t kMaxThreads = (int64_t)1 << 32;   // a launch has fewer
-
-// kBlocks blocks of 16 channels a workgroup, kSplit waves for each.
-template <int kBlocks, int kSplit>
-struct FewRows {
-  static constexpr int kWaves = kBlocks * kSplit, kThreads = 64 * kWaves;
-  static constexpr int kChannels = 16 * kBlocks;
-};
-
-// This wave's part of the 16 x 16 product of W rows n0 .. and x rows m0 .., summed over
-// the waves of the block into the first of them.
-template <int kBlocks, int kSplit>
-__device__ __forceinline__ i32x4 few_rows_sum(const ProjI8Args& a, int64_t n0, int64_t m0, int wave,
-                                              int lane, i32x4 (*part)[64]) {
-  const int block = wave % kBlocks, split = wave / kBlocks;
-  const int lr = lane & 15, g = lane >> 4;
-  // Rows past the last are the last one's: in bounds, and never stored.
-  const int64_t n = min(n0 + 16 * block + lr, (int64_t)a.n_total - 1);
-  const int64_t m = min(m0 + lr, (int64_t)a.out.seq_len - 1);
-  const int8_t* wp = a.w + n * a.ldw + 32 * g;
-  const int8_t* xp = a.x + m * a.ldx + 32 * g;
-  i32x4 acc = {0, 0, 0, 0};
-  for (int k = kStepBytes * split; k < a.in; k += kStepBytes * kSplit) {
-    const i32x4 w0 = *reinterpret_cast<const i32x4*>(wp + k);
-    const i32x4 w1 = *reinterpret_cast<const i32x4*>(wp + k + 16);
-    const i32x4 x0 = *reinterpret_cast<const i32x4*>(xp + k);
-    const i32x4 x1 = *reinterpret_cast<const i32x4*>(xp + k + 16);
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, x0, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, x1, acc, 0, 0, 0);
-  }
-  if (kSplit > 1) {
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (split == 0) {
-#pragma unroll
-      for (int s = 1; s < kSplit; s++) acc += part[wave + kBlocks * s][lane];
-    }
-  }
-  return acc;
-}
-
-// Sums of channels 4g .. +3 of a token, with their scales.
-__device__ __forceinline__ f32x4 scaled(const i32x4& acc, float xs, const float (&ws)[4]) {
-  f32x4 y;
-#pragma unroll
-  for (int i = 0; i < 4; i++) y[i] = (float)acc[i] * xs * ws[i];
-  return y;
-}
-
-template <int kSplit>
-__global__ __launch_bounds__(64 * kSplit) void proj_i8_rows_kernel(ProjI8Args a) {
-  __shared__ i32x4 part[kSplit][64];
-  const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int tiles_n = (a.n_total + 15) / 16;
-  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * kRowTokens;
-  const int64_t n0 = (int64_t)(blockIdx.x % tiles_n) * 16;
-  const i32x4 acc = few_rows_sum<1, kSplit>(a, n0, m0, wave, lane, part);
-  const int64_t m = m0 + lr, n = n0 + 4 * g;
-  if (wave != 0 || m >= a.out.seq_len || n >= a.n_total) return;
-  float ws[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) ws[i] = a.w_scale[min(n + i, (int64_t)a.n_total - 1)];
-  const f32x4 y = scaled(acc, a.x_scale[m], ws);
-  uint16_t* dst = a.out.q_out + m * a.out.ldo + n;
-  const u32x2 v = {cvt_pk(y[0], y[1]), cvt_pk(y[2], y[3])};
-  if (a.wide && n + 4 <= a.n_total) {
-    *reinterpret_cast<u32x2*>(dst) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (n + i < a.n_total) dst[i] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
-  }
-}
-
-// One head and 16 tokens: eight blocks of 16 channels.
-template <int kSplit, int kMode, int kHl, bool kPlain>
-__global__ __launch_bounds__(512 * kSplit) void qkv_proj_i8_rows_kernel(ProjI8Args a) {
-  constexpr int kBlocks = kHeadDim / 16;
-  __shared__ i32x4 part[kBlocks * kSplit][64];
-  __shared__ __attribute__((aligned(16))) uint16_t rows[kRowTokens * kHeadDim];
-  constexpr int kRowWaves = kRowTokens / 8;
-  __shared__ __attribute__((aligned(16))) RopeEntry tables[kRowWaves * 512];
-  const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int heads3 = 3 * a.out.heads;
-  const int m0 = (int)(blockIdx.x / heads3) * kRowTokens;
-  const int n0 = (int)(blockIdx.x % heads3) * kHeadDim;
-  if (m0 >= a.out.seq_len) {
-    zero_tile_rows<kRowTokens, kHeadDim, 512 * kSplit>(a.out, threadIdx.x, m0, n0);
-    return;
-  }
-  const i32x4 acc = few_rows_sum<kBlocks, kSplit>(a, n0, m0, wave, lane, part);
-  if (wave < kBlocks) {
-    const f32x4 w4 = *reinterpret_cast<const f32x4*>(a.w_scale + n0 + 16 * wave + 4 * g);
-    const float ws[4] = {w4[0], w4[1], w4[2], w4[3]};
-    const f32x4 y = scaled(acc, a.x_scale[min(m0 + lr, a.out.seq_len - 1)], ws);
-    const int chunk = 2 * wave + (g >> 1);
-    *reinterpret_cast<u32x2*>(rows + lr * kHeadDim + (chunk ^ e_swz(lr)) * 8 + 4 * (g & 1)) =
-        u32x2{cvt_pk(y[0], y[1]), cvt_pk(y[2], y[3])};
-  }
-  __syncthreads();
-  if (wave < kRowWaves)
-    finish_tile_rows<kRowTokens, kHeadDim, kRowWaves, kMode, kHl, kPlain, false>(
-        a.out, rows, tables, wave, lane, m0, n0);
-}
-
-template <int kSplit>
-int launch_qkv_rows(const ProjI8Args& a, int32_t rounding, bool plain, hipStream_t st) {
-  const int64_t tiles = (int64_t)(a.out.seq_pad / kRowTokens) * 3 * a.out.heads;
-  H3_REQUIRE(tiles * 512 * kSplit < kMaxThreads, H3HIP_EINVAL,
-             "too many rows x heads for one launch (%lld tiles)", (long long)tiles);
-  const dim3 grid((unsigned)tiles), block(512 * kSplit);
-  constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32;
-  if (plain)
-    qkv_proj_i8_rows_kernel<kSplit, kRef, 8, true><<<grid, block, 0, st>>>(a);
-  else if (rounding == kRef && a.out.rot == 128)
-    qkv_proj_i8_rows_kernel<kSplit, kRef, 8, false><<<grid, block, 0, st>>>(a);
-  else if (rounding == kRef)
-    qkv_proj_i8_rows_kernel<kSplit, kRef, 6, false><<<grid, block, 0, st>>>(a);
-  else if (a.out.rot == 128)
-    qkv_proj_i8_rows_kernel<kSplit, kF32, 8, false><<<grid, block, 0, st>>>(a);
-  else
-    qkv_proj_i8_rows_kernel<kSplit, kF32, 6, false><<<grid, block, 0, st>>>(a);
-  return check_launch("qkv_proj_i8_rows_kernel");
-}
-
 constexpr int kMaxIn = 131071;                      // x 128 x 128 stays below 2^31
 constexpr int64_t kMaxStride = ((int64_t)1 << 31) / 256;
 
@@ -214,16 +76,7 @@ extern "C" int h3hip_proj_i8(const void* x, int64_t ldx, const float* x_scale, c
   a.in = in_features;
   a.n_total = out_features;
   a.wide = ldy % 8 == 0 && aligned(y, 16);
-  const ProjI8Tile tile = pick_proj_i8_tile(rows, rows, out_features, false);
-  if (tile != ProjI8Tile::kRows)
-    return launch_proj_i8_gemm(a, tile, H3HIP_ROUND_REFERENCE, true, true, as_stream(stream));
-  constexpr int kSplit = 8;
-  const int64_t tiles = (((int64_t)rows + kRowTokens - 1) / kRowTokens) *
-                        (((int64_t)out_features + 15) / 16);
-  H3_REQUIRE(tiles * 64 * kSplit < kMaxThreads, H3HIP_EINVAL,
-             "too many rows x channels for one launch (%d x %d)", rows, out_features);
-  proj_i8_rows_kernel<kSplit><<<dim3((unsigned)tiles), 64 * kSplit, 0, as_stream(stream)>>>(a);
-  return check_launch("proj_i8_rows_kernel");
+  return launch_proj_i8_gemm(a, H3HIP_ROUND_REFERENCE, true, true, as_stream(stream));
 }
 
 extern "C" int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scale, const void* w,
@@ -276,8 +129,5 @@ extern "C" int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scal
   a.ldw = ldw;
   a.in = hidden;
   a.n_total = 3 * heads * kHeadDim;
-  const ProjI8Tile tile = pick_proj_i8_tile(seq_len, seq_pad, a.n_total, true);
-  if (tile != ProjI8Tile::kRows)
-    return launch_proj_i8_gemm(a, tile, rounding, plain, false, as_stream(stream));
-  return launch_qkv_rows<2>(a, rounding, plain, as_stream(stream));
+  return launch_proj_i8_gemm(a, rounding, plain, false, as_stream(stream));
 }

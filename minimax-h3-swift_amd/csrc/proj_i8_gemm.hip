@@ -1,5 +1,4 @@
-// The int8 projections' GEMM on four waves: tiles of W x^T for any number of rows
-// beyond the few that proj_i8.hip takes.
+// The int8 projections' GEMM on four waves: tiles of W x^T, from one row to any number.
 //
 // The loop is the bf16 GEMM's (proj_gemm.hip has its layout and why it is four waves)
 // with v_mfma_i32_16x16x64_i8 in place of the bf16 product: twice the operations for the
@@ -11,6 +10,7 @@
 // LDS as token rows, and from there what the bf16 projections do (proj_rows.h).
 #include "gemm_i8_loop.inc"
 #include "proj_i8.h"
+#include "proj_i8_tile.h"
 #include "proj_rows.h"
 #include "tile_order.h"
 
@@ -37,11 +37,11 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) {
 
 // One tile shape: its LDS and its reduction loop, from lane offsets and scalars
 // to accumulators.
-template <int kNA, int kMB>
+template <int kNA, int kMB, bool kPair>
 struct Shape;
-#define H3_SHAPE(NA, MB, NAME)                                                               \
+#define H3_SHAPE(NA, MB, PAIR, NAME)                                                         \
   template <>                                                                                \
-  struct Shape<NA, MB> {                                                                     \
+  struct Shape<NA, MB, PAIR> {                                                                  \
     static constexpr int kLds = H3_GEMM_I8_LDS_##NAME, kBases = H3_GEMM_I8_BASES_##NAME;       \
     static __device__ __forceinline__ void reduce(i32x32 (&c)[kAccs<NA, MB>], const int* ra,   \
                                                   const int* rb, const int* xv, const int* wv, \
@@ -54,15 +54,20 @@ struct Shape;
                    : H3_GEMM_I8_CLOBBERS_##NAME);                                            \
     }                                                                                        \
   };
-H3_SHAPE(8, 8, 256x256)
-H3_SHAPE(8, 7, 256x224)
-H3_SHAPE(8, 6, 256x192)
-H3_SHAPE(8, 5, 256x160)
-H3_SHAPE(8, 4, 256x128)
-H3_SHAPE(4, 6, 128x192)
-H3_SHAPE(4, 5, 128x160)
-H3_SHAPE(4, 4, 128x128)
-H3_SHAPE(4, 2, 128x64)
+H3_SHAPE(8, 8, false, 256x256)
+H3_SHAPE(8, 7, false, 256x224)
+H3_SHAPE(8, 6, false, 256x192)
+H3_SHAPE(8, 5, false, 256x160)
+H3_SHAPE(8, 4, false, 256x128)
+H3_SHAPE(4, 6, false, 128x192)
+H3_SHAPE(4, 5, false, 128x160)
+H3_SHAPE(4, 4, false, 128x128)
+H3_SHAPE(4, 4, true, 128x128p)
+H3_SHAPE(4, 2, true, 128x64p)
+H3_SHAPE(4, 1, true, 128x32p)
+H3_SHAPE(2, 2, true, 64x64p)
+H3_SHAPE(1, 2, true, 32x64p)
+H3_SHAPE(1, 1, true, 32x32p)
 
 // Scales of channels n .. n + 3.
 __device__ __forceinline__ f32x4 channel_scales(const ProjI8Args& a, int64_t n, bool whole) {
@@ -73,8 +78,22 @@ __device__ __forceinline__ f32x4 channel_scales(const ProjI8Args& a, int64_t n, 
   return s;
 }
 
-// The tile's epilogue. Accumulator (na, mb) of lane (g, lr): channels
-// 16 (kNA wc + na) + 4g .. +3 of token 16 (kMB wt + mb) + lr.
+// Accumulators of channels 16 (kNA wc + na) + 4g .. +3 and token 16 (kMB wt + mb) + lr, with
+// their scales, in bf16.
+template <int kNA, int kMB>
+__device__ __forceinline__ u32x2 scaled_block(const i32x32 (&c)[kAccs<kNA, kMB>], int na, int mb,
+                                              float xs, const f32x4& ws) {
+  const int e = 4 * (kMB * na + mb);
+  const i32x32& v = c[e / 32];
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) y[i] = (float)v[e % 32 + i] * xs * ws[i];
+  return u32x2{cvt_pk(y[0], y[1]), cvt_pk(y[2], y[3])};
+}
+
+// The tile's epilogue. Tiles of a head or two go through LDS as token rows; narrower ones,
+// whose few rows gain nothing from that, are stored from the accumulators, 32 bytes of a
+// row at a time.
 template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>
 __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
                                             const i32x32 (&c)[kAccs<kNA, kMB>], int wave, int lane,
@@ -85,36 +104,58 @@ __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
 #pragma unroll
   for (int mb = 0; mb < kMB; mb++)
     xs[mb] = a.x_scale[min(m0 + 16 * (kMB * wt + mb) + lr, a.out.seq_len - 1)];
-  // bf16 token rows of the whole tile in LDS; chunk c (16 bytes) of row r sits
-  // at c ^ e_swz(r), within its head.
+  if constexpr (kChannels < 128) {
+    static_assert(kOut, "heads are written through LDS");
 #pragma unroll
-  for (int na = 0; na < kNA; na++) {
-    const f32x4 ws = channel_scales(a, n0 + 16 * (kNA * wc + na) + 4 * g, !kOut);
-    const int chunk = 2 * (kNA * wc + na) + (g >> 1);
-    const int pos = (chunk & 16) | ((chunk & 15) ^ e_swz(lr));
+    for (int na = 0; na < kNA; na++) {
+      const int64_t n = n0 + 16 * (kNA * wc + na) + 4 * g;
+      if (n >= a.n_total) continue;
+      const f32x4 ws = channel_scales(a, n, false);
 #pragma unroll
-    for (int mb = 0; mb < kMB; mb++) {
-      const int r = 16 * (kMB * wt + mb) + lr, e = 4 * (kMB * na + mb);
-      const i32x32& v = c[e / 32];
-      float y[4];
+      for (int mb = 0; mb < kMB; mb++) {
+        const int m = m0 + 16 * (kMB * wt + mb) + lr;
+        if (m >= a.out.seq_len) continue;
+        uint16_t* dst = a.out.q_out + (int64_t)m * a.out.ldo + n;
+        const u32x2 y = scaled_block<kNA, kMB>(c, na, mb, xs[mb], ws);
+        if (a.wide && n + 4 <= a.n_total) {
+          *reinterpret_cast<u32x2*>(dst) = y;
+        } else {
 #pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = (float)v[e % 32 + i] * xs[mb] * ws[i];
-      *reinterpret_cast<u32x2*>(lds + r * kChannels + pos * 8 + 4 * (g & 1)) =
-          u32x2{cvt_pk(y[0], y[1]), cvt_pk(y[2], y[3])};
+          for (int i = 0; i < 4; i++)
+            if (n + i < a.n_total) dst[i] = (uint16_t)(y[i / 2] >> (16 * (i & 1)));
+        }
+      }
     }
+  } else {
+    // bf16 token rows of the whole tile in LDS; chunk c (16 bytes) of row r sits
+    // at c ^ e_swz(r), within its head.
+#pragma unroll
+    for (int na = 0; na < kNA; na++) {
+      const f32x4 ws = channel_scales(a, n0 + 16 * (kNA * wc + na) + 4 * g, !kOut);
+      const int chunk = 2 * (kNA * wc + na) + (g >> 1);
+      const int pos = (chunk & 16) | ((chunk & 15) ^ e_swz(lr));
+#pragma unroll
+      for (int mb = 0; mb < kMB; mb++)
+        *reinterpret_cast<u32x2*>(lds + (16 * (kMB * wt + mb) + lr) * kChannels + pos * 8 +
+                                  4 * (g & 1)) = scaled_block<kNA, kMB>(c, na, mb, xs[mb], ws);
+    }
+    __syncthreads();
+    finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, kOut>(
+        a.out, lds, reinterpret_cast<RopeEntry*>(lds + kTokens * kChannels), wave, lane, m0, n0,
+        a.wide != 0);
+    // The last token tile's workgroup also owns the rows behind its tile.
+    if (!kOut && m0 + kTokens >= a.out.seq_len)
+      zero_rows<kChannels, kThreads>(a.out, 64 * wave + lane, m0 + kTokens, n0);
   }
-  __syncthreads();
-  finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, kOut>(
-      a.out, lds, reinterpret_cast<RopeEntry*>(lds + kTokens * kChannels), wave, lane, m0, n0,
-      a.wide != 0);
 }
 
-template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>
-__global__ __launch_bounds__(kThreads, 1) void proj_i8_gemm_kernel(ProjI8Args a) {
-  using S = Shape<kNA, kMB>;
+template <int kNA, int kMB, bool kPair, int kMode, int kHl, bool kPlain, bool kOut>
+__global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_i8_gemm_kernel(ProjI8Args a) {
+  using S = Shape<kNA, kMB, kPair>;
   constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
-  static_assert(S::kLds >= 2 * kTokens * kChannels + kWaves * kRowTableLds,
+  static_assert(kChannels < 128 || S::kLds >= 2 * kTokens * kChannels + kWaves * kRowTableLds,
                 "the epilogue's rows and tables fit in the rings");
+  static_assert(!kPair || 2 * S::kLds <= 163840, "two workgroups' rings fit a CU");
   __shared__ __attribute__((aligned(16))) uint16_t lds[S::kLds / 2];
 
   const int lane = threadIdx.x & 63;
@@ -125,10 +166,6 @@ __global__ __launch_bounds__(kThreads, 1) void proj_i8_gemm_kernel(ProjI8Args a)
   if (slot >= order.length(xcd)) return;
   const uint32_t tile = order.tile(xcd, slot);
   const int m0 = (int)(tile >> 16) * kTokens, n0 = (int)(tile & 0xffff) * kChannels;
-  if (!kOut && m0 >= a.out.seq_len) {
-    zero_tile_rows<kTokens, kChannels, kThreads>(a.out, threadIdx.x, m0, n0);
-    return;
-  }
 
   const int lr = lane & 15, g = lane >> 4;
   const uint32_t lds_base = uniform((uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t*)lds);
@@ -171,43 +208,53 @@ __global__ __launch_bounds__(kThreads, 1) void proj_i8_gemm_kernel(ProjI8Args a)
   finish_tile<kNA, kMB, kMode, kHl, kPlain, kOut>(a, lds, c, wave, lane2, m0, n0);
 }
 
-template <int kNA, int kMB>
+template <int kNA, int kMB, bool kPair>
 int launch(ProjI8Args a, int32_t rounding, bool plain, bool out, hipStream_t st) {
-  const ProjGrid g = proj_i8_grid(out ? a.out.seq_len : a.out.seq_pad, a.n_total, 32 * kMB, 32 * kNA);
+  const ProjGrid g = proj_i8_grid(a.out.seq_len, a.n_total, 32 * kMB, 32 * kNA);
   a.out.tiles_m = g.order.tiles_m;
   a.out.chunk = g.order.chunk;
   const dim3 grid(kOrderXcds * g.longest);
   constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32;
-  if (out)
-    proj_i8_gemm_kernel<kNA, kMB, kRef, 8, true, true><<<grid, kThreads, 0, st>>>(a);
-  else if (plain)
-    proj_i8_gemm_kernel<kNA, kMB, kRef, 8, true, false><<<grid, kThreads, 0, st>>>(a);
-  else if (rounding == kRef && a.out.rot == 128)
-    proj_i8_gemm_kernel<kNA, kMB, kRef, 8, false, false><<<grid, kThreads, 0, st>>>(a);
-  else if (rounding == kRef)
-    proj_i8_gemm_kernel<kNA, kMB, kRef, 6, false, false><<<grid, kThreads, 0, st>>>(a);
-  else if (a.out.rot == 128)
-    proj_i8_gemm_kernel<kNA, kMB, kF32, 8, false, false><<<grid, kThreads, 0, st>>>(a);
-  else
-    proj_i8_gemm_kernel<kNA, kMB, kF32, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+  if (out) {
+    proj_i8_gemm_kernel<kNA, kMB, kPair, kRef, 8, true, true><<<grid, kThreads, 0, st>>>(a);
+  } else if constexpr (kNA >= 4) {
+    if (plain)
+      proj_i8_gemm_kernel<kNA, kMB, kPair, kRef, 8, true, false><<<grid, kThreads, 0, st>>>(a);
+    else if (rounding == kRef && a.out.rot == 128)
+      proj_i8_gemm_kernel<kNA, kMB, kPair, kRef, 8, false, false><<<grid, kThreads, 0, st>>>(a);
+    else if (rounding == kRef)
+      proj_i8_gemm_kernel<kNA, kMB, kPair, kRef, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+    else if (a.out.rot == 128)
+      proj_i8_gemm_kernel<kNA, kMB, kPair, kF32, 8, false, false><<<grid, kThreads, 0, st>>>(a);
+    else
+      proj_i8_gemm_kernel<kNA, kMB, kPair, kF32, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+  }
   return check_launch("proj_i8_gemm_kernel");
 }
 
 }  // namespace
 
-int launch_proj_i8_gemm(const ProjI8Args& a, ProjI8Tile tile, int32_t rounding, bool plain, bool out,
+int launch_proj_i8_gemm(const ProjI8Args& a, int32_t rounding, bool plain, bool out,
                         hipStream_t stream) {
-  switch (tile) {
-    case ProjI8Tile::k256x256: return launch<8, 8>(a, rounding, plain, out, stream);
-    case ProjI8Tile::k256x224: return launch<8, 7>(a, rounding, plain, out, stream);
-    case ProjI8Tile::k256x192: return launch<8, 6>(a, rounding, plain, out, stream);
-    case ProjI8Tile::k256x160: return launch<8, 5>(a, rounding, plain, out, stream);
-    case ProjI8Tile::k256x128: return launch<8, 4>(a, rounding, plain, out, stream);
-    case ProjI8Tile::k128x192: return launch<4, 6>(a, rounding, plain, out, stream);
-    case ProjI8Tile::k128x160: return launch<4, 5>(a, rounding, plain, out, stream);
-    case ProjI8Tile::k128x128: return launch<4, 4>(a, rounding, plain, out, stream);
-    default: return launch<4, 2>(a, rounding, plain, out, stream);
+  switch (pick_proj_i8_tile(a.out.seq_len, a.n_total, a.in / kStep, !out)) {
+    case ProjI8Tile::k256x256: return launch<8, 8, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x224: return launch<8, 7, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x192: return launch<8, 6, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x160: return launch<8, 5, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k256x128: return launch<8, 4, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x192: return launch<4, 6, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x160: return launch<4, 5, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x128: return launch<4, 4, false>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x128p: return launch<4, 4, true>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x64p: return launch<4, 2, true>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k128x32p: return launch<4, 1, true>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k64x64p: return launch<2, 2, true>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k32x64p: return launch<1, 2, true>(a, rounding, plain, out, stream);
+    case ProjI8Tile::k32x32p: return launch<1, 1, true>(a, rounding, plain, out, stream);
+    default: break;
   }
+  set_error("too many rows or channels for one launch (%d x %d)", a.out.seq_len, a.n_total);
+  return H3HIP_EINVAL;
 }
 
 }  // namespace h3hip

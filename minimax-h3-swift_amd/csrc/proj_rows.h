@@ -22,18 +22,18 @@ __device__ __forceinline__ void store_row_chunk(uint16_t* dst, u32x4 v, int left
     if (e < left) dst[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
 }
 
-// Zeros into rows m0 .. of the heads of channels n0 ..: a tile of padding rows only.
-template <int kTokens, int kChannels, int kThreads>
-__device__ __forceinline__ void zero_tile_rows(const ProjArgs& a, int tid, int m0, int n0) {
+// Zeros into rows m0 .. seq_pad - 1 of the heads of channels n0 .., by kThreads threads.
+template <int kChannels, int kThreads>
+__device__ __forceinline__ void zero_rows(const ProjArgs& a, int tid, int m0, int n0) {
   constexpr int kHead = 128, kChunks = kHead / 8;
   const int inner = a.heads * kHead, part = n0 / inner;
-  const int head0 = (n0 - part * inner) / kHead;
   uint16_t* out = part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
-  for (int i = tid; i < kTokens * (kChannels / 8); i += kThreads) {
-    const int head = head0 + i / (kTokens * kChunks), r = i / kChunks % kTokens;
-    if (m0 + r < a.seq_pad)
-      *reinterpret_cast<u32x4*>(out + ((int64_t)head * a.seq_pad + m0 + r) * kHead +
-                                8 * (i % kChunks)) = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll 1
+  for (int nh = 0; nh < kChannels / kHead; nh++) {
+    uint16_t* head = out + (int64_t)((n0 - part * inner) / kHead + nh) * a.seq_pad * kHead;
+    for (int r = m0 + tid / kChunks; r < a.seq_pad; r += kThreads / kChunks)
+      *reinterpret_cast<u32x4*>(head + (int64_t)r * kHead + 8 * (tid % kChunks)) =
+          u32x4{0u, 0u, 0u, 0u};
   }
 }
 

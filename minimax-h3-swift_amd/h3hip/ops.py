@@ -331,17 +331,20 @@ def quant_rows(x: torch.Tensor, out=None):
 
 
 def _int8_operands(x, x_scale, w, w_scale):
-    """Checks the operands of an int8 projection; returns (ldx, ldw)."""
+    """Checks the operands of an int8 projection; returns (device, S, K, N, ldx, ldw)."""
     ldx, ldw = _rows("x", x, torch.int8), _rows("w", w, torch.int8)
-    if w.shape[1] != x.shape[1]:
-        raise ValueError(f"w must be [out, {x.shape[1]}], got {tuple(w.shape)}")
+    S, K = x.shape
+    N, k = w.shape
+    if k != K:
+        raise ValueError(f"w must be [out, {K}], got {tuple(w.shape)}")
     device = x.device
-    _require_same_device(device, w=w)
-    _vector("x_scale", x_scale, x.shape[0], device)
-    _vector("w_scale", w_scale, w.shape[0], device)
+    if w.device != device:
+        raise ValueError(f"w must be on {device}, got {w.device}")
+    _vector("x_scale", x_scale, S, device)
+    _vector("w_scale", w_scale, N, device)
     if not x.is_cuda:
         raise ValueError("x must be a GPU tensor (no host fallback exists)")
-    return ldx, ldw
+    return device, S, K, N, ldx, ldw
 
 
 def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -351,17 +354,16 @@ def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     x: [S, K] int8 and x_scale: [S] fp32, w: [N, K] int8 and w_scale: [N] fp32, as
     quant_rows() makes them (K a multiple of 128). Returns y [S, N] bf16 (or writes
     ``out``, any row stride), or None when declined."""
-    ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
-    (S, K), N = x.shape, w.shape[0]
+    device, S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
     if out is None:
-        out = torch.empty((S, N), dtype=torch.bfloat16, device=x.device)
+        out = torch.empty((S, N), dtype=torch.bfloat16, device=device)
         ldy = N
     else:
         ldy = _rows("out", out, torch.bfloat16)
         if out.shape != (S, N):
             raise ValueError(f"out must be [{S}, {N}], got {tuple(out.shape)}")
-        _require_same_device(x.device, out=out)
-    rc = _run(L.lib().h3hip_proj_i8, x.device, x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(),
+        _require_same_device(device, out=out)
+    rc = _run(L.lib().h3hip_proj_i8, device, x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(),
               ldw, w_scale.data_ptr(), K, N, S, out.data_ptr(), ldy)
     return None if rc == L.DECLINED else out
 
@@ -375,21 +377,19 @@ def qkv_proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     [3*heads*head_dim, hidden]): the QKV product with the Q/K norm + RoPE in its
     epilogue. Returns (q, k, v) as [heads, seq_pad, head_dim] bf16, or None when the
     geometry is declined."""
-    ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
-    S, K = x.shape
-    device = x.device
-    if w.shape[0] != 3 * heads * head_dim:
+    device, S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
+    if N != 3 * heads * head_dim:
         raise ValueError(f"w must be [{3 * heads * head_dim}, {K}], got {tuple(w.shape)}")
     seq_pad = seq_pad or (S + L.TILE - 1) // L.TILE * L.TILE
     if q_gamma is None and k_gamma is None:
         rot, gq, gk, tab = head_dim, None, None, None
     else:
-        rot = _check_norm_rope(S, head_dim, q_gamma, k_gamma, table, rounding)
-        _require_same_device(device, q_gamma=q_gamma, k_gamma=k_gamma, table=table)
+        rot = _check_norm_rope(device, S, head_dim, q_gamma, k_gamma, table, rounding)
         gq, gk, tab = q_gamma.data_ptr(), k_gamma.data_ptr(), table.data_ptr()
     shape = (heads, seq_pad, head_dim)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(3))
+        # One allocation: three take 2 us more of a call that can be as short as 20.
+        out = torch.empty((3, *shape), dtype=torch.bfloat16, device=device).unbind(0)
     else:
         out = tuple(out)
         for t in out:
@@ -401,16 +401,16 @@ def qkv_proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     return None if rc == L.DECLINED else out
 
 
-def _check_norm_rope(S, head_dim, q_gamma, k_gamma, table, rounding) -> int:
+def _check_norm_rope(device, S, head_dim, q_gamma, k_gamma, table, rounding) -> int:
     """Checks what the Q/K norm and rotation read; returns rot."""
     for name, t in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
-        if t is None or t.shape != (head_dim,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous [{head_dim}]")
-        _require_gpu_bf16(name, t)
+        if (t is None or t.dtype != torch.bfloat16 or t.shape != (head_dim,)
+                or not t.is_contiguous() or t.device != device):
+            raise ValueError(f"{name} must be contiguous bfloat16 [{head_dim}] on {device}")
     dt = torch.bfloat16 if rounding == L.ROUND_REFERENCE else torch.float32
-    if (table is None or not table.is_cuda or table.dtype != dt or not table.is_contiguous()
-            or table.dim() != 4 or table.shape[0] < S or table.shape[2:] != (2, 2)):
-        raise ValueError(f"table must be a contiguous {dt} [>= {S}, rot/2, 2, 2] GPU tensor "
+    if (table is None or table.dtype != dt or table.dim() != 4 or table.shape[0] < S
+            or table.shape[2:] != (2, 2) or not table.is_contiguous() or table.device != device):
+        raise ValueError(f"table must be a contiguous {dt} [>= {S}, rot/2, 2, 2] tensor on {device} "
                          "(rope_table() with the same rounding mode)")
     return 2 * table.shape[1]
 

@@ -9,6 +9,14 @@ from _int8 import bits16, check_product, int8_operands, product64
 
 pytestmark = pytest.mark.gpu
 
+# One size for each tile shape (rows, in, out), with rows and channels that end inside a
+# tile; test_proj_i8_tile_host.py checks which shape each one takes.
+SHAPES = [("256x256", 6001, 1024, 5000), ("256x224", 2500, 256, 5000), ("256x192", 2001, 384, 5000),
+          ("256x160", 2500, 256, 3500), ("256x128", 641, 384, 9000), ("128x192", 500, 128, 9000),
+          ("128x160", 801, 128, 5000), ("128x128", 385, 640, 5000), ("128x128p", 385, 128, 5000),
+          ("128x64p", 100, 128, 9000), ("128x32p", 1, 128, 9000), ("64x64p", 1, 256, 9000),
+          ("32x64p", 33, 128, 5000), ("32x32p", 1, 128, 100)]
+
 
 @pytest.mark.parametrize("S,K,N", [
     (1, 128, 1), (1, 128, 16), (1, 5120, 5120), (2, 128, 17), (15, 256, 128), (16, 384, 130),
@@ -23,6 +31,21 @@ def test_against_64_bits(h3, S, K, N):
     torch.cuda.synchronize()
     assert y.shape == (S, N) and y.dtype == torch.bfloat16
     check_product(y, product64(x, xs, w, ws))
+
+
+@pytest.mark.parametrize("shape,S,K,N", SHAPES, ids=[s[0] for s in SHAPES])
+def test_every_tile_shape(h3, shape, S, K, N):
+    """At two lengths of reduction that take it, into rows that are and are not on 16 bytes;
+    nothing past a row's channels or the last row is written."""
+    from h3hip import ops
+    x, xs, w, ws = int8_operands(S, K, N, S + N)
+    want = product64(x, xs, w, ws)
+    for ldy, first in ((N + 8 - N % 8, 0), (N + 3, 1)):
+        buf = torch.full(((S + 1) * ldy + first,), 7.0, dtype=torch.bfloat16, device="cuda")
+        rows = buf[first:].view(S + 1, ldy)
+        note(f"proj_i8 {shape} S={S} K={K} N={N} ldy={ldy}")
+        check_product(ops.proj_i8(x, xs, w, ws, out=rows[:S, :N]), want)
+        assert (rows[S] == 7.0).all() and (rows[:, N:] == 7.0).all() and (buf[:first] == 7.0).all()
 
 
 @pytest.mark.parametrize("S,K,N,ldx,ldw,ldy,first", [

@@ -35,7 +35,16 @@ def _gammas(seed):
             for _ in range(2)]
 
 
-CASES = [(1, 128, 1, 128), (1, 5120, 40, 128), (5, 256, 3, 96), (16, 384, 2, 128),
+# One size for each tile shape (rows, hidden, heads, rot); test_proj_i8_tile_host.py
+# checks which shape each one takes.
+SHAPES = [("256x256", 1000, 384, 40, 128), ("256x224", 801, 256, 40, 96),
+          ("256x192", 641, 384, 40, 96), ("256x160", 1000, 256, 24, 128),
+          ("256x128", 385, 384, 40, 96), ("128x192", 500, 128, 24, 96),
+          ("128x160", 257, 128, 40, 128), ("128x128", 129, 640, 40, 96),
+          ("128x128p", 129, 128, 40, 128), ("128x64p", 65, 128, 40, 96),
+          ("128x32p", 1, 128, 1, 96)]
+CASES = [s[1:] for s in SHAPES]
+CASES += [(1, 128, 1, 128), (1, 5120, 40, 128), (5, 256, 3, 96), (16, 384, 2, 128),
          (17, 640, 2, 96), (33, 128, 5, 128), (65, 1152, 4, 96), (128, 256, 1, 96),
          (129, 512, 4, 128), (300, 1024, 7, 128), (637, 5120, 40, 128), (1151, 5376, 56, 96),
          (700, 1152, 40, 128), (2100, 256, 6, 128)]
@@ -98,6 +107,23 @@ def test_fp32_rounding_against_64_bits(h3, S, K, H, rot):
         worst = float((d / bound).max())
         print(f"qkv_proj_i8 {'qk'[i]}: worst error / bound {worst:.3f}", flush=True)
         assert worst <= 1.0
+
+
+def test_more_padding_than_a_tile(h3):
+    """seq_pad may lie far behind seq_len: every row between is zero, in all three parts."""
+    from h3hip import ops
+    for S, K, H in ((3, 256, 3), (300, 384, 4), (1100, 640, 6)):
+        x, xs, w, ws = int8_operands(S, K, 3 * H * D, S)
+        gq, gk = _gammas(2)
+        table = _rope(S, 128, 1)[3]
+        pad = (S + 127) // 128 * 128 + 640
+        out = [torch.full((H, pad, D), 9.0, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+        note(f"qkv_proj_i8 S={S} seq_pad={pad}")
+        ops.qkv_proj_i8(x, xs, w, ws, gq, gk, table, heads=H, seq_pad=pad, rounding=1, out=out)
+        near = ops.qkv_proj_i8(x, xs, w, ws, gq, gk, table, heads=H, rounding=1)
+        for a, b in zip(out, near):
+            assert not a[:, S:].any()
+            assert (bits16(a[:, :S]) == bits16(b[:, :S])).all()
 
 
 def test_rows_of_zeros_and_nan(h3):
