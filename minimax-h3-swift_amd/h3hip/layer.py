@@ -16,6 +16,10 @@ out-projection -- a plain GEMM -- on the projection kernel's main loop
 (h3hip_out_proj), or on hipBLASLt when that kernel declines the shape. Q and K
 come out head-major and V is read in place, so no relayout copy runs between
 the stages.
+
+With ``projection="int8"`` both projections run on int8 operands with scales for
+each token and output channel (h3hip_quant_rows, h3hip_qkv_proj_i8,
+h3hip_proj_i8): the weights are rounded once, the activations in every call.
 """
 from __future__ import annotations
 
@@ -62,6 +66,24 @@ class RopeState:
         return cls.build(pos, axis, inv, head_dim, rounding)
 
 
+@dataclass
+class Int8Weight:
+    """A projection's weight rounded to int8 once: [out, in padded to a multiple of 128]
+    int8 rows with an fp32 scale each."""
+    values: torch.Tensor
+    scale: torch.Tensor
+    in_features: int
+
+    @classmethod
+    def round(cls, weight: torch.Tensor) -> "Int8Weight":
+        """weight: [out, in] bf16 on the GPU."""
+        return cls(*ops.quant_rows(weight), weight.shape[1])
+
+    @property
+    def shape(self):
+        return self.values.shape[0], self.in_features
+
+
 class AttentionLayer:
     """One DiT attention layer (DiTBlock.swift:262-359).
 
@@ -69,16 +91,24 @@ class AttentionLayer:
     out_weight: [hidden, heads*head_dim] bf16; q_gamma, k_gamma: [head_dim] bf16
     (qNorm, kNorm). ``projection`` picks the QKV path: "fused" (h3hip_qkv_proj)
     or "hipblaslt" (GEMM + h3hip_qk_norm_rope); either falls back to the other
-    when its kernel declines the geometry."""
+    when its kernel declines the geometry. "int8" runs both projections on int8
+    operands (qkv_weight and out_weight are rounded here, or given as Int8Weight;
+    the bf16 ones are not kept, so nothing is fallen back to)."""
 
     def __init__(self, qkv_weight, out_weight, q_gamma, k_gamma, *, heads: int,
                  head_dim: int = 128, eps: float = 1e-5, backend: H3AttentionBackend | None = None,
                  projection: str = "hipblaslt"):
-        if projection not in ("fused", "hipblaslt"):
-            raise ValueError(f"projection must be 'fused' or 'hipblaslt', got {projection!r}")
+        if projection not in ("fused", "hipblaslt", "int8"):
+            raise ValueError("projection must be 'fused', 'hipblaslt' or 'int8', got "
+                             f"{projection!r}")
         inner = heads * head_dim
         if qkv_weight.shape[0] != 3 * inner or out_weight.shape[1] != inner:
             raise ValueError("weights do not match heads * head_dim")
+        if projection == "int8":
+            qkv_weight, out_weight = (w if isinstance(w, Int8Weight) else Int8Weight.round(w)
+                                      for w in (qkv_weight, out_weight))
+        elif isinstance(qkv_weight, Int8Weight) or isinstance(out_weight, Int8Weight):
+            raise ValueError("an Int8Weight needs projection='int8'")
         self.qkv_weight, self.out_weight = qkv_weight, out_weight
         self.q_gamma, self.k_gamma = q_gamma, k_gamma
         self.heads, self.head_dim, self.eps = heads, head_dim, eps
@@ -108,6 +138,13 @@ class AttentionLayer:
         v = qkv[:, 2 * inner:].view(S, self.heads, self.head_dim).transpose(0, 1)
         return r[0][:, :S], r[1][:, :S], v
 
+    def _project_int8(self, x, rope: RopeState, seq_pad: int):
+        w, S = self.qkv_weight, x.shape[0]
+        r = ops.qkv_proj_i8(*ops.quant_rows(x), w.values, w.scale, self.q_gamma, self.k_gamma,
+                            rope.table, heads=self.heads, head_dim=self.head_dim, eps=self.eps,
+                            seq_pad=seq_pad, rounding=rope.rounding)
+        return None if r is None else tuple(t[:, :S] for t in r)
+
     def _attend(self, q, k, v, context: AttentionContext | None):
         """AttentionLayer.sdpa (DiTBlock.swift:280-328) on [H, S, D] views:
         the backend only with a context; a decline runs dense SDPA."""
@@ -133,20 +170,26 @@ class AttentionLayer:
     def __call__(self, x: torch.Tensor, rope: RopeState | None,
                  context: AttentionContext | None = None) -> torch.Tensor:
         """x: [S, hidden] bf16 -> [S, hidden] bf16."""
-        if x.dim() != 2:
-            raise ValueError("x must be [S, hidden] (the packed-row layout)")
+        if x.dim() != 2 or x.shape[1] != self.qkv_weight.shape[1]:
+            raise ValueError(f"x must be [S, {self.qkv_weight.shape[1]}] (the packed-row layout), "
+                             f"got {tuple(x.shape)}")
         S = x.shape[0]
         if rope is None:
             rope = RopeState.identity(S, self.head_dim, x.device)
         seq_pad = ((S + L.TILE - 1) // L.TILE) * L.TILE
-        first, second = ((self._project_fused, self._project_hipblaslt)
-                         if self.projection == "fused"
-                         else (self._project_hipblaslt, self._project_fused))
-        qkv = first(x, rope, seq_pad) or second(x, rope, seq_pad)
+        paths = {"fused": (self._project_fused, self._project_hipblaslt),
+                 "hipblaslt": (self._project_hipblaslt, self._project_fused),
+                 "int8": (self._project_int8,)}[self.projection]
+        qkv = None
+        for project in paths:
+            qkv = qkv or project(x, rope, seq_pad)
         if qkv is None:
             raise NotImplementedError(
                 f"no kernel takes head_dim {self.head_dim} / rot {rope.rot} / heads {self.heads}")
         merged = self._attend(*qkv, context)
+        if self.projection == "int8":
+            return ops.proj_i8(*ops.quant_rows(merged), self.out_weight.values,
+                               self.out_weight.scale)
         y = ops.out_proj(merged, self.out_weight)
         if y is None:       # a width the kernel declines: hipBLASLt's GEMM
             y = torch.mm(merged, self.out_weight.t())
