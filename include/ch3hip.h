@@ -296,7 +296,7 @@ int h3hip_quant_rows(const void* x, int64_t ldx, int32_t rows, int32_t cols, voi
                      float* scale, void* stream);
 
 /* A projection on int8 operands with scales for each token and channel:
- *   y[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n]
+ *   y[m, n] = ((sum_k x[m, k] w[n, k]) * w_scale[n]) * x_scale[m]
  * The sum is exact (int32); it, and its products with the scales, are rounded to
  * fp32, the result once to bf16. The int8 form of h3hip_out_proj, for any number of
  * rows (0 and 1 too) and any width.

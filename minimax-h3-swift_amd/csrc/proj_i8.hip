@@ -1,6 +1,6 @@
 // The int8 projections' entry points (kernel: proj_i8_gemm.hip).
 //
-//   y[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n]
+//   y[m, n] = ((sum_k x[m, k] w[n, k]) w_scale[n]) x_scale[m]
 //
 // with x and w int8 and the sum exact in int32 (in_features up to 131,071, whatever
 // the values): what rounds is the sum's conversion to fp32, the two products with

@@ -79,7 +79,8 @@ __device__ __forceinline__ f32x4 channel_scales(const ProjI8Args& a, int64_t n, 
 }
 
 // Accumulators of channels 16 (kNA wc + na) + 4g .. +3 and token 16 (kMB wt + mb) + lr, with
-// their scales, in bf16.
+// their scales, in bf16. The channel's scale first: a weight's is moderate, a token's may be
+// near either end of fp32, and so nothing overflows between that the result does not.
 template <int kNA, int kMB>
 __device__ __forceinline__ u32x2 scaled_block(const i32x32 (&c)[kAccs<kNA, kMB>], int na, int mb,
                                               float xs, const f32x4& ws) {
@@ -87,7 +88,7 @@ __device__ __forceinline__ u32x2 scaled_block(const i32x32 (&c)[kAccs<kNA, kMB>]
   const i32x32& v = c[e / 32];
   float y[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) y[i] = (float)v[e % 32 + i] * xs * ws[i];
+  for (int i = 0; i < 4; i++) y[i] = (float)v[e % 32 + i] * ws[i] * xs;
   return u32x2{cvt_pk(y[0], y[1]), cvt_pk(y[2], y[3])};
 }
 

@@ -81,8 +81,14 @@ inline ProjI8Tile pick_proj_i8_tile(int tokens, int channels, int steps, bool he
     if ((heads && channels / 3 % std::max(s.channels, 128) != 0) || (heads && s.channels < 128) ||
         !proj_i8_fits(tokens, channels, s))
       continue;
+    const float round = s.per_tile + s.per_step * (float)steps;
+    // A round for each tile a CU gets at least: most shapes need no look at their lists.
+    const int tiles_m = (int)(((int64_t)tokens + s.tokens - 1) / s.tokens);
+    const int tiles_n = (int)(((int64_t)channels + s.channels - 1) / s.channels);
+    const int least = (tiles_m * tiles_n + 32 * kOrderXcds - 1) / (32 * kOrderXcds);
+    if (tile != ProjI8Tile::kNone && s.start + (float)least * round >= best) continue;
     const int rounds = proj_i8_grid(tokens, channels, s.tokens, s.channels).rounds;
-    const float cost = s.start + (float)rounds * (s.per_tile + s.per_step * (float)steps);
+    const float cost = s.start + (float)rounds * round;
     if (tile == ProjI8Tile::kNone || cost < best) {
       best = cost;
       tile = s.tile;

@@ -55,7 +55,7 @@ struct RowTable {
   static constexpr int kLoads = kRef ? kHl / 2 : kHl;
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   u32x4 ref[kRef ? kLoads : 1];
-  f32x2 f32[kRef ? 1 : kLoads];
+  f32x4 f32[kRef ? 1 : kLoads];
 
   __device__ __forceinline__ void load(const void* table, int64_t row, int j) {
     constexpr int kHalf = 8 * kHl;
@@ -64,9 +64,9 @@ struct RowTable {
 #pragma unroll
       for (int t = 0; t < kLoads; t++) ref[t] = *reinterpret_cast<const u32x4*>(p + 64 * t);
     } else {
-      const float* p = static_cast<const float*>(table) + (row * kHalf + j) * 4 + 2;
+      const f32x4* p = static_cast<const f32x4*>(table) + row * kHalf + j;
 #pragma unroll
-      for (int t = 0; t < kLoads; t++) f32[t] = *reinterpret_cast<const f32x2*>(p + 32 * t);
+      for (int t = 0; t < kLoads; t++) f32[t] = p[8 * t];
     }
   }
   static __device__ __forceinline__ int unit(int b, int rg) { return ((b >> 2) & 1) | (rg & 1) << 1; }
@@ -75,13 +75,13 @@ struct RowTable {
     RopeEntry* mine = lds + 64 * rg;
 #pragma unroll
     for (int t = 0; t < kLoads; t++) {
-      if constexpr (kRef) {   // entries 16t + 2j, + 1; words 1 and 3 are (s, c)
+      if constexpr (kRef) {   // entries 16t + 2j, + 1: (c, -s, s, c) bf16 each
         const int b = 2 * t + (j >> 2);
-        const f32x4 v = {bf16_hi(ref[t][1]), bf16_lo(ref[t][1]), bf16_hi(ref[t][3]),
+        const f32x4 v = {bf16_lo(ref[t][0]), bf16_lo(ref[t][1]), bf16_lo(ref[t][2]),
                          bf16_lo(ref[t][3])};
         *reinterpret_cast<f32x4*>(mine + 8 * (b ^ rg) + 2 * ((j & 3) ^ unit(b, rg))) = v;
-      } else {                // entry 8t + j, (s, c)
-        const f32x2 v = {f32[t][1], f32[t][0]};
+      } else {                // entry 8t + j
+        const f32x2 v = {f32[t][0], f32[t][2]};
         *reinterpret_cast<f32x2*>(mine + 8 * (t ^ rg) + 2 * ((j >> 1) ^ unit(t, rg)) + (j & 1)) = v;
       }
     }

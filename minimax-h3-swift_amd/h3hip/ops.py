@@ -281,15 +281,15 @@ def _require_same_device(device: torch.device, **others):
 
 
 def _rows(name: str, t: torch.Tensor, dtype) -> int:
-    """The row stride of a 2-D tensor whose rows are contiguous (of a single row, any that
-    covers it)."""
+    """The row stride of a 2-D tensor whose rows are contiguous. A single row has none that
+    matters: the least that covers it and keeps the next one aligned."""
     if t.dtype != dtype or t.dim() != 2:
         raise ValueError(f"{name} must be 2-D {dtype}, got {t.dim()}-D {t.dtype}")
     ld, step = t.stride()
     rows, cols = t.shape
     if step != 1 and cols > 1:
         raise ValueError(f"{name} must have unit column stride, got strides {t.stride()}")
-    return ld if rows > 1 else max(ld, cols)
+    return ld if rows > 1 else (cols + 15) // 16 * 16
 
 
 def _vector(name: str, t: torch.Tensor, n: int, device: torch.device):
@@ -349,7 +349,7 @@ def _int8_operands(x, x_scale, w, w_scale):
 
 def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
             out: torch.Tensor | None = None):
-    """A projection on int8 operands: y = (x . w^T) * x_scale[:, None] * w_scale.
+    """A projection on int8 operands: y = (x . w^T) * w_scale * x_scale[:, None].
 
     x: [S, K] int8 and x_scale: [S] fp32, w: [N, K] int8 and w_scale: [N] fp32, as
     quant_rows() makes them (K a multiple of 128). Returns y [S, N] bf16 (or writes

@@ -96,6 +96,39 @@ def test_scales_that_are_zero_or_nan(h3, S):
     check_product(torch.where(nan, 0, y), product64(x, xs, w, ws).masked_fill(nan, 0.0))
 
 
+@pytest.mark.parametrize("S", [2, 300])
+def test_scales_at_the_ends_of_fp32(h3, S):
+    """A token's scale of any magnitude with a weight's: only the result's own overflow and
+    underflow show. (sum * w_scale stays in fp32's range: at most 2^31 * 0.1.)"""
+    from h3hip import ops
+    x, xs, w, ws = int8_operands(S, 512, 300, 5)
+    xs[0], xs[1] = 3.0e38, 1.5e-38
+    note(f"proj_i8 extreme scales S={S}")
+    y = ops.proj_i8(x, xs, w, ws)
+    want = product64(x, xs, w, ws)
+    top = torch.finfo(torch.bfloat16).max
+    over = want.abs() > top * 1.01
+    assert torch.isinf(y[over]).all() and (torch.sign(y[over]) == torch.sign(want[over])).all()
+    near = (want.abs() > top * 0.99) | over
+    check_product(torch.where(near, 0, y), want.masked_fill(near, 0.0))
+
+
+def test_a_single_row_of_any_stride(h3):
+    """One row has no row stride: whatever its tensor says is taken."""
+    from h3hip import ops
+    x, xs, w, ws = int8_operands(1, 256, 100, 6)
+    odd = torch.as_strided(x, (1, 256), (1000003, 1))
+    y = torch.empty((40,) * 3, dtype=torch.bfloat16, device="cuda").view(-1)[8:108]
+    note("proj_i8 single rows")
+    want = bits16(ops.proj_i8(x, xs, w, ws))
+    got = ops.proj_i8(odd, xs, w, ws, out=torch.as_strided(y, (1, 100), (3, 1)))
+    assert (bits16(got) == want).all()
+    b = torch.randn((1, 777), device="cuda").to(torch.bfloat16)
+    q, s = ops.quant_rows(b)
+    q2, s2 = ops.quant_rows(torch.as_strided(b, (1, 777), (5, 1)))
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
 def test_no_rows(h3):
     from h3hip import ops
     _, _, w, ws = int8_operands(1, 128, 40, 1)
