@@ -69,14 +69,35 @@ H3_SHAPE(2, 2, true, 64x64p)
 H3_SHAPE(1, 2, true, 32x64p)
 H3_SHAPE(1, 1, true, 32x32p)
 
-// Scales of channels n .. n + 3.
-__device__ __forceinline__ f32x4 channel_scales(const ProjI8Args& a, int64_t n, bool whole) {
-  if (whole || n + 4 <= a.n_total) return *reinterpret_cast<const f32x4*>(a.w_scale + n);
-  f32x4 s;
+// A lane's scales: of token 16 (kMB wt + mb) + lr, and of channels 16 (kNA wc + na) + 4g .. +3.
+template <int kNA, int kMB>
+struct Scales {
+  float x[kMB];
+  f32x4 w[kNA];
+  // Past the last token or channel: the last one's, unused. heads: every channel exists.
+  __device__ __forceinline__ void load_x(const ProjI8Args& a, int wave, int lane, int m0) {
+    const int wt = wave & 1, lr = lane & 15;
 #pragma unroll
-  for (int i = 0; i < 4; i++) s[i] = a.w_scale[min(n + i, (int64_t)a.n_total - 1)];
-  return s;
-}
+    for (int mb = 0; mb < kMB; mb++)
+      x[mb] = a.x_scale[min(m0 + 16 * (kMB * wt + mb) + lr, a.out.seq_len - 1)];
+  }
+  __device__ __forceinline__ void load_w(const ProjI8Args& a, int wave, int lane, int n0,
+                                         bool heads) {
+    const int wc = wave >> 1, g = lane >> 4;
+    if (heads || n0 + 32 * kNA <= a.n_total) {
+#pragma unroll
+      for (int na = 0; na < kNA; na++)
+        w[na] = *reinterpret_cast<const f32x4*>(a.w_scale + n0 + 16 * (kNA * wc + na) + 4 * g);
+      return;
+    }
+#pragma unroll
+    for (int na = 0; na < kNA; na++) {
+      const int n = n0 + 16 * (kNA * wc + na) + 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[na][i] = a.w_scale[min(n + i, a.n_total - 1)];
+    }
+  }
+};
 
 // Accumulators of channels 16 (kNA wc + na) + 4g .. +3 and token 16 (kMB wt + mb) + lr, with
 // their scales, in bf16. The channel's scale first: a weight's is moderate, a token's may be
@@ -97,27 +118,23 @@ __device__ __forceinline__ u32x2 scaled_block(const i32x32 (&c)[kAccs<kNA, kMB>]
 // row at a time.
 template <int kNA, int kMB, int kMode, int kHl, bool kPlain, bool kOut>
 __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
-                                            const i32x32 (&c)[kAccs<kNA, kMB>], int wave, int lane,
-                                            int m0, int n0) {
+                                            const i32x32 (&c)[kAccs<kNA, kMB>],
+                                            const Scales<kNA, kMB>& s, int wave, int lane, int m0,
+                                            int n0) {
   constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
   const int wc = wave >> 1, wt = wave & 1, lr = lane & 15, g = lane >> 4;
-  float xs[kMB];
-#pragma unroll
-  for (int mb = 0; mb < kMB; mb++)
-    xs[mb] = a.x_scale[min(m0 + 16 * (kMB * wt + mb) + lr, a.out.seq_len - 1)];
   if constexpr (kChannels < 128) {
     static_assert(kOut, "heads are written through LDS");
 #pragma unroll
     for (int na = 0; na < kNA; na++) {
       const int64_t n = n0 + 16 * (kNA * wc + na) + 4 * g;
       if (n >= a.n_total) continue;
-      const f32x4 ws = channel_scales(a, n, false);
 #pragma unroll
       for (int mb = 0; mb < kMB; mb++) {
         const int m = m0 + 16 * (kMB * wt + mb) + lr;
         if (m >= a.out.seq_len) continue;
         uint16_t* dst = a.out.q_out + (int64_t)m * a.out.ldo + n;
-        const u32x2 y = scaled_block<kNA, kMB>(c, na, mb, xs[mb], ws);
+        const u32x2 y = scaled_block<kNA, kMB>(c, na, mb, s.x[mb], s.w[na]);
         if (a.wide && n + 4 <= a.n_total) {
           *reinterpret_cast<u32x2*>(dst) = y;
         } else {
@@ -132,13 +149,12 @@ __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
     // at c ^ e_swz(r), within its head.
 #pragma unroll
     for (int na = 0; na < kNA; na++) {
-      const f32x4 ws = channel_scales(a, n0 + 16 * (kNA * wc + na) + 4 * g, !kOut);
       const int chunk = 2 * (kNA * wc + na) + (g >> 1);
       const int pos = (chunk & 16) | ((chunk & 15) ^ e_swz(lr));
 #pragma unroll
       for (int mb = 0; mb < kMB; mb++)
         *reinterpret_cast<u32x2*>(lds + (16 * (kMB * wt + mb) + lr) * kChannels + pos * 8 +
-                                  4 * (g & 1)) = scaled_block<kNA, kMB>(c, na, mb, xs[mb], ws);
+                                  4 * (g & 1)) = scaled_block<kNA, kMB>(c, na, mb, s.x[mb], s.w[na]);
     }
     __syncthreads();
     finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, kOut>(
@@ -199,6 +215,12 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_i8_gemm_kernel(P
   const uint32_t steps = uniform((uint32_t)(a.in / kStep));
   const uint32_t m0w = uniform(lds_base + 1024u * kNA * wave);
   const uint32_t m0x = uniform(lds_base + 1024u * kMB * wave);
+  // The scales arrive during the loop; the tokens' of the largest tile would be spilled
+  // across it.
+  constexpr bool kEarlyX = kNA * kMB < 64;
+  Scales<kNA, kMB> scales;
+  if (kEarlyX) scales.load_x(a, wave, lane, m0);
+  scales.load_w(a, wave, lane, n0, !kOut);
   i32x32 c[kAccs<kNA, kMB>];
   S::reduce(c, ra, rb, xv, wv, x_lo, x_hi, x_rec, w_lo, w_hi, w_rec, steps, m0x, m0w);
 
@@ -206,7 +228,8 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_i8_gemm_kernel(P
   // be spilled across it.
   int lane2;
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane2));
-  finish_tile<kNA, kMB, kMode, kHl, kPlain, kOut>(a, lds, c, wave, lane2, m0, n0);
+  if (!kEarlyX) scales.load_x(a, wave, lane2, m0);
+  finish_tile<kNA, kMB, kMode, kHl, kPlain, kOut>(a, lds, c, scales, wave, lane2, m0, n0);
 }
 
 template <int kNA, int kMB, bool kPair>

@@ -127,12 +127,14 @@ __device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16
     oa = *reinterpret_cast<const u32x4*>(row + ((chunk_a ^ e_swz(r & 15)) * 8));
     ob = *reinterpret_cast<const u32x4*>(row + ((chunk_b ^ e_swz(r & 15)) * 8));
   };
+  // Whether every channel of the tile is a channel of the output, on 16 bytes.
+  const bool full = !kRagged || (wide && n0 + kChannels <= a.n_out);
   auto store_row = [&](int r, int nh, bool valid, u32x4 oa, u32x4 ob) __attribute__((always_inline)) {
     const int m = m0 + r;
     if (!valid) oa = ob = u32x4{0u, 0u, 0u, 0u};
     uint16_t* dst = kOut ? a.q_out + (int64_t)m * a.ldo + n0 + nh * kHead
                          : out + ((int64_t)(head0 + nh) * a.seq_pad + m) * kHead;
-    if constexpr (kRagged) {
+    if (kRagged && !full) {
       if (valid) {
         const int left = a.n_out - n0 - nh * kHead;
         store_row_chunk(dst + 8 * chunk_a, oa, left - 8 * chunk_a, wide);
