@@ -286,8 +286,7 @@ int h3hip_out_proj(const void* x, int64_t ldx, const void* w, int64_t ldw, int32
  *   quotient is rounded before), scale[m] = a / 127 in fp32, so that x is about
  *   q * scale. A row of zeros has scale 0. A row that holds an infinity or a NaN has
  *   scale NaN and values 0: every product with it is NaN.
- *   x:     device bf16 [rows, cols], row stride ldx elements, any alignment (rows on
- *          16 bytes, i.e. x 16-byte aligned and ldx a multiple of 8, load widest).
+ *   x:     device bf16 [rows, cols], row stride ldx elements; rows may begin anywhere.
  *   q:     device int8 [rows, cols_pad], cols_pad = ceil(cols/128)*128, row stride
  *          ldq bytes (a multiple of 16); 16-byte aligned; columns past cols are zeros.
  *   scale: device fp32 [rows].
@@ -304,8 +303,8 @@ int h3hip_quant_rows(const void* x, int64_t ldx, int32_t rows, int32_t cols, voi
  *      [out_features, in_features], row stride ldw bytes: as h3hip_quant_rows writes
  *      them (any values, -128 too; 16-byte aligned, strides multiples of 16).
  *   x_scale: device fp32 [rows]; w_scale: device fp32 [out_features], 16-byte aligned.
- *   y: device bf16 [rows, out_features], row stride ldy elements; nothing else is
- *      written. Any alignment (16 bytes and ldy a multiple of 8 store widest).
+ *   y: device bf16 [rows, out_features], row stride ldy elements; rows may begin
+ *      anywhere, and nothing else is written.
  * Operands may pass 4 GiB; 256 rows of x or w must stay below 2 GiB.
  * Declines unless in_features is a multiple of 128 (h3hip_quant_rows pads with
  * zeros) and at most 131,071. No workspace; can be captured into a graph. */

@@ -15,7 +15,6 @@ struct ProjI8Args {
   const float* __restrict__ w_scale;    // [n_total]
   int64_t ldx, ldw;
   int32_t in, n_total;
-  int32_t wide;   // token-major output: rows and row stride allow 16-byte stores
 };
 
 // Launches proj_i8_gemm_kernel on the tile shape that suits the sizes (proj_i8_gemm.hip).

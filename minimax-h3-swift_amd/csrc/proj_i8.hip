@@ -75,7 +75,6 @@ extern "C" int h3hip_proj_i8(const void* x, int64_t ldx, const float* x_scale, c
   a.ldw = ldw;
   a.in = in_features;
   a.n_total = out_features;
-  a.wide = ldy % 8 == 0 && aligned(y, 16);
   return launch_proj_i8_gemm(a, H3HIP_ROUND_REFERENCE, true, true, as_stream(stream));
 }
 

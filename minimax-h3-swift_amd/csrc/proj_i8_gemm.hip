@@ -135,8 +135,8 @@ __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
         if (m >= a.out.seq_len) continue;
         uint16_t* dst = a.out.q_out + (int64_t)m * a.out.ldo + n;
         const u32x2 y = scaled_block<kNA, kMB>(c, na, mb, s.x[mb], s.w[na]);
-        if (a.wide && n + 4 <= a.n_total) {
-          *reinterpret_cast<u32x2*>(dst) = y;
+        if (n + 4 <= a.n_total) {
+          *reinterpret_cast<u32x2_any*>(dst) = y;
         } else {
 #pragma unroll
           for (int i = 0; i < 4; i++)
@@ -158,8 +158,7 @@ __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
     }
     __syncthreads();
     finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, kOut>(
-        a.out, lds, reinterpret_cast<RopeEntry*>(lds + kTokens * kChannels), wave, lane, m0, n0,
-        a.wide != 0);
+        a.out, lds, reinterpret_cast<RopeEntry*>(lds + kTokens * kChannels), wave, lane, m0, n0);
     // The last token tile's workgroup also owns the rows behind its tile.
     if (!kOut && m0 + kTokens >= a.out.seq_len)
       zero_rows<kChannels, kThreads>(a.out, 64 * wave + lane, m0 + kTokens, n0);

@@ -11,10 +11,10 @@
 
 namespace h3hip {
 
-// Up to 8 channels of a token-major row; wide: the address is 16-byte aligned.
-__device__ __forceinline__ void store_row_chunk(uint16_t* dst, u32x4 v, int left, bool wide) {
-  if (wide && left >= 8) {
-    *reinterpret_cast<u32x4*>(dst) = v;
+// Up to 8 channels of a token-major row, which may begin anywhere.
+__device__ __forceinline__ void store_row_chunk(uint16_t* dst, u32x4 v, int left) {
+  if (left >= 8) {
+    *reinterpret_cast<u32x4_any*>(dst) = v;
     return;
   }
 #pragma unroll
@@ -100,13 +100,12 @@ constexpr int kRowTableLds = 8 * 64 * sizeof(RopeEntry);   // bytes of a wave
 // prologue's 8-lane layout, head after head, so that a row's rotation entries are
 // fetched once. kHl = rot / 16 (8-channel chunks per rotation half);
 // kPlain: every part unchanged; kOut: token-major with row stride ldo; kRagged (with
-// kOut): any output width and row stride, wide saying that the row stride and the
-// output's address allow 16-byte stores. tables: kRowTableLds bytes for each wave.
+// kOut): any output width, row stride and address. tables: kRowTableLds bytes for each wave.
 template <int kTokens, int kChannels, int kRowWaves, int kMode, int kHl, bool kPlain, bool kOut,
           bool kRagged = false>
 __device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16_t* lds,
                                                  RopeEntry* tables, int wave, int lane, int m0,
-                                                 int n0, bool wide = true) {
+                                                 int n0) {
   constexpr int kHead = 128;
   constexpr int kHeads = kChannels / kHead, kRows = kTokens / kRowWaves;
   static_assert(kRows % 8 == 0, "whole passes");
@@ -127,8 +126,8 @@ __device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16
     oa = *reinterpret_cast<const u32x4*>(row + ((chunk_a ^ e_swz(r & 15)) * 8));
     ob = *reinterpret_cast<const u32x4*>(row + ((chunk_b ^ e_swz(r & 15)) * 8));
   };
-  // Whether every channel of the tile is a channel of the output, on 16 bytes.
-  const bool full = !kRagged || (wide && n0 + kChannels <= a.n_out);
+  // Whether every channel of the tile is a channel of the output.
+  const bool full = !kRagged || n0 + kChannels <= a.n_out;
   auto store_row = [&](int r, int nh, bool valid, u32x4 oa, u32x4 ob) __attribute__((always_inline)) {
     const int m = m0 + r;
     if (!valid) oa = ob = u32x4{0u, 0u, 0u, 0u};
@@ -137,12 +136,13 @@ __device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16
     if (kRagged && !full) {
       if (valid) {
         const int left = a.n_out - n0 - nh * kHead;
-        store_row_chunk(dst + 8 * chunk_a, oa, left - 8 * chunk_a, wide);
-        store_row_chunk(dst + 8 * chunk_b, ob, left - 8 * chunk_b, wide);
+        store_row_chunk(dst + 8 * chunk_a, oa, left - 8 * chunk_a);
+        store_row_chunk(dst + 8 * chunk_b, ob, left - 8 * chunk_b);
       }
     } else if (!kOut || valid) {
-      *reinterpret_cast<u32x4*>(dst + 8 * chunk_a) = oa;
-      *reinterpret_cast<u32x4*>(dst + 8 * chunk_b) = ob;
+      using Chunk = std::conditional_t<kRagged, u32x4_any, u32x4>;
+      *reinterpret_cast<Chunk*>(dst + 8 * chunk_a) = oa;
+      *reinterpret_cast<Chunk*>(dst + 8 * chunk_b) = ob;
     }
   };
   // Passes of 8 rows; head-major rows end at seq_pad, a multiple of 8.

@@ -45,13 +45,13 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
                                                                 __builtin_bit_cast(u16x2, b)));
 }
 
-// A lane's 16 elements from column k on, zeros past cols. kWide: the row begins on 16 bytes.
-template <bool kWide>
-__device__ __forceinline__ void load_chunk(const uint16_t* row, int k, int cols, uint32_t (&v)[8]) {
-  if (kWide && k + kLaneElems <= cols) {
+// A lane's 16 elements from column k on, zeros past cols. Rows may begin anywhere: gfx950
+// loads 16 bytes from any address.
+__device__ __forceinline__ void load_chunk(const uint16_t* row, int64_t k, int cols, uint32_t (&v)[8]) {
+  if (k + kLaneElems <= cols) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(row + k + 8 * h);
+      const u32x4 w = *reinterpret_cast<const u32x4_any*>(row + k + 8 * h);
 #pragma unroll
       for (int i = 0; i < 4; i++) v[4 * h + i] = w[i];
     }
@@ -87,7 +87,7 @@ __device__ __forceinline__ uint32_t code(float x, const RowScale& r) {
 }
 
 // The lane's 16 codes into 16 bytes at k, as far as the padded row goes.
-__device__ __forceinline__ void store_chunk(int8_t* row, int k, int cols_pad,
+__device__ __forceinline__ void store_chunk(int8_t* row, int64_t k, int cols_pad,
                                             const uint32_t (&v)[8], const RowScale& r) {
   if (k >= cols_pad) return;
   u32x4 o;
@@ -104,7 +104,7 @@ __device__ __forceinline__ void store_chunk(int8_t* row, int k, int cols_pad,
 }
 
 // kChunks: chunks of the row, held in registers; 0: any number, read twice.
-template <int kChunks, bool kWide>
+template <int kChunks>
 __global__ __launch_bounds__(64 * kWavesWg) void quant_rows_kernel(QuantArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t m = (int64_t)blockIdx.x * kWavesWg +
@@ -113,17 +113,20 @@ __global__ __launch_bounds__(64 * kWavesWg) void quant_rows_kernel(QuantArgs a) 
   const uint16_t* row = a.x + m * a.ldx;
   int8_t* out = a.q + m * a.ldq;
   const int k0 = kLaneElems * lane;
-  uint32_t v[kChunks ? kChunks : 1][8];
+  constexpr int kHeld = kChunks ? kChunks : 4;   // chunks in registers at once
+  uint32_t v[kHeld][8];
   uint32_t top2 = 0;
   if constexpr (kChunks != 0) {
 #pragma unroll
-    for (int c = 0; c < kChunks; c++) load_chunk<kWide>(row, k0 + c * kChunk, a.cols, v[c]);
+    for (int c = 0; c < kChunks; c++) load_chunk(row, k0 + c * kChunk, a.cols, v[c]);
 #pragma unroll
     for (int c = 0; c < kChunks; c++) top2 = chunk_max(v[c], top2);
   } else {
-    for (int64_t k = k0; k < a.cols; k += kChunk) {
-      load_chunk<kWide>(row, (int)k, a.cols, v[0]);
-      top2 = chunk_max(v[0], top2);
+    for (int64_t k = 0; k < a.cols; k += kHeld * kChunk) {
+#pragma unroll
+      for (int c = 0; c < kHeld; c++) load_chunk(row, k + k0 + c * kChunk, a.cols, v[c]);
+#pragma unroll
+      for (int c = 0; c < kHeld; c++) top2 = chunk_max(v[c], top2);
     }
   }
   uint32_t top = max(top2 & 0xffffu, top2 >> 16);
@@ -148,20 +151,21 @@ __global__ __launch_bounds__(64 * kWavesWg) void quant_rows_kernel(QuantArgs a) 
 #pragma unroll
     for (int c = 0; c < kChunks; c++) store_chunk(out, k0 + c * kChunk, a.cols_pad, v[c], r);
   } else {
-    for (int64_t k = k0; k < a.cols_pad; k += kChunk) {
-      load_chunk<kWide>(row, (int)k, a.cols, v[0]);
-      store_chunk(out, (int)k, a.cols_pad, v[0], r);
+    for (int64_t k = 0; k < a.cols_pad; k += kHeld * kChunk) {
+#pragma unroll
+      for (int c = 0; c < kHeld; c++) load_chunk(row, k + k0 + c * kChunk, a.cols, v[c]);
+#pragma unroll
+      for (int c = 0; c < kHeld; c++) store_chunk(out, k + k0 + c * kChunk, a.cols_pad, v[c], r);
     }
   }
 }
 
-template <bool kWide>
 void launch(const QuantArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((a.rows + (int64_t)kWavesWg - 1) / kWavesWg));
   const int chunks = (a.cols_pad + kChunk - 1) / kChunk;
   switch (chunks) {
 #define H3_CHUNKS(N) \
-  case N: quant_rows_kernel<N, kWide><<<grid, 64 * kWavesWg, 0, st>>>(a); break
+  case N: quant_rows_kernel<N><<<grid, 64 * kWavesWg, 0, st>>>(a); break
     H3_CHUNKS(1);
     H3_CHUNKS(2);
     H3_CHUNKS(3);
@@ -171,7 +175,7 @@ void launch(const QuantArgs& a, hipStream_t st) {
     H3_CHUNKS(7);
     H3_CHUNKS(8);
 #undef H3_CHUNKS
-    default: quant_rows_kernel<0, kWide><<<grid, 64 * kWavesWg, 0, st>>>(a);
+    default: quant_rows_kernel<0><<<grid, 64 * kWavesWg, 0, st>>>(a);
   }
 }
 
@@ -197,9 +201,6 @@ extern "C" int h3hip_quant_rows(const void* x, int64_t ldx, int32_t rows, int32_
              H3HIP_EINVAL, "x must be 2-byte, q 16-byte and scale 4-byte aligned");
   const QuantArgs a{static_cast<const uint16_t*>(x), static_cast<int8_t*>(q), scale, ldx, ldq,
                     rows, cols, cols_pad};
-  if (ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0)
-    launch<true>(a, as_stream(stream));
-  else
-    launch<false>(a, as_stream(stream));
+  launch(a, as_stream(stream));
   return check_launch("quant_rows_kernel");
 }

@@ -330,21 +330,30 @@ def quant_rows(x: torch.Tensor, out=None):
     return q, scale
 
 
+_I8, _F32 = torch.int8, torch.float32
+
+
 def _int8_operands(x, x_scale, w, w_scale):
     """Checks the operands of an int8 projection; returns (device, S, K, N, ldx, ldw)."""
-    ldx, ldw = _rows("x", x, torch.int8), _rows("w", w, torch.int8)
-    S, K = x.shape
-    N, k = w.shape
-    if k != K:
-        raise ValueError(f"w must be [out, {K}], got {tuple(w.shape)}")
-    device = x.device
-    if w.device != device:
-        raise ValueError(f"w must be on {device}, got {w.device}")
-    _vector("x_scale", x_scale, S, device)
-    _vector("w_scale", w_scale, N, device)
-    if not x.is_cuda:
-        raise ValueError("x must be a GPU tensor (no host fallback exists)")
-    return device, S, K, N, ldx, ldw
+    if x.dim() == w.dim() == 2:
+        (S, K), (N, k) = x.shape, w.shape
+        (ldx, step), (ldw, step_w) = x.stride(), w.stride()
+        device = x.device
+        if (x.dtype is _I8 and w.dtype is _I8 and x_scale.dtype is _F32 and w_scale.dtype is _F32
+                and k == K and step == 1 and step_w == 1 and x_scale.shape == (S,)
+                and w_scale.shape == (N,) and x_scale.is_contiguous() and w_scale.is_contiguous()
+                and x.is_cuda and w.device == device and x_scale.device == device
+                and w_scale.device == device):
+            return device, S, K, N, (ldx if S > 1 else K), (ldw if N > 1 else K)
+    # What of it is refused, one by one.
+    _rows("x", x, _I8)
+    _rows("w", w, _I8)
+    if w.shape[1] != x.shape[1]:
+        raise ValueError(f"w must be [out, {x.shape[1]}], got {tuple(w.shape)}")
+    _require_same_device(x.device, w=w)
+    _vector("x_scale", x_scale, x.shape[0], x.device)
+    _vector("w_scale", w_scale, w.shape[0], x.device)
+    raise ValueError("x must be a GPU tensor of more than one column (no host fallback exists)")
 
 
 def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
