@@ -74,17 +74,16 @@ template <int kNA, int kMB>
 struct Scales {
   float x[kMB];
   f32x4 w[kNA];
-  // Past the last token or channel: the last one's, unused. heads: every channel exists.
+  // Past the last token or channel: the last one's, unused.
   __device__ __forceinline__ void load_x(const ProjI8Args& a, int wave, int lane, int m0) {
     const int wt = wave & 1, lr = lane & 15;
 #pragma unroll
     for (int mb = 0; mb < kMB; mb++)
       x[mb] = a.x_scale[min(m0 + 16 * (kMB * wt + mb) + lr, a.out.seq_len - 1)];
   }
-  __device__ __forceinline__ void load_w(const ProjI8Args& a, int wave, int lane, int n0,
-                                         bool heads) {
+  __device__ __forceinline__ void load_w(const ProjI8Args& a, int wave, int lane, int n0) {
     const int wc = wave >> 1, g = lane >> 4;
-    if (heads || n0 + 32 * kNA <= a.n_total) {
+    if (n0 + 32 * kNA <= a.n_total) {
 #pragma unroll
       for (int na = 0; na < kNA; na++)
         w[na] = *reinterpret_cast<const f32x4*>(a.w_scale + n0 + 16 * (kNA * wc + na) + 4 * g);
@@ -157,7 +156,7 @@ __device__ __forceinline__ void finish_tile(const ProjI8Args& a, uint16_t* lds,
                                   4 * (g & 1)) = scaled_block<kNA, kMB>(c, na, mb, s.x[mb], s.w[na]);
     }
     __syncthreads();
-    finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, kOut>(
+    finish_tile_rows<kTokens, kChannels, kWaves, kMode, kHl, kPlain, kOut, true>(
         a.out, lds, reinterpret_cast<RopeEntry*>(lds + kTokens * kChannels), wave, lane, m0, n0);
     // The last token tile's workgroup also owns the rows behind its tile.
     if (!kOut && m0 + kTokens >= a.out.seq_len)
@@ -219,7 +218,7 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_i8_gemm_kernel(P
   constexpr bool kEarlyX = kNA * kMB < 64;
   Scales<kNA, kMB> scales;
   if (kEarlyX) scales.load_x(a, wave, lane, m0);
-  scales.load_w(a, wave, lane, n0, !kOut);
+  scales.load_w(a, wave, lane, n0);
   i32x32 c[kAccs<kNA, kMB>];
   S::reduce(c, ra, rb, xv, wv, x_lo, x_hi, x_rec, w_lo, w_hi, w_rec, steps, m0x, m0w);
 

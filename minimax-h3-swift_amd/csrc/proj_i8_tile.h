@@ -67,7 +67,7 @@ inline ProjGrid proj_i8_grid(int tokens, int channels, int tile_tokens, int tile
 }
 
 // The shape whose launch takes least; kNone if none fits one. heads: the output is
-// written by heads, so a tile holds whole heads of one of Q, K and V.
+// written by heads, so a tile holds whole ones.
 //
 // The constants are least squares over 440 sizes (1 to 18,102 tokens, 777 to 15,360
 // channels, 3 to 56 steps, without norm) of every shape on MI355X, whose times they give to
@@ -78,9 +78,7 @@ inline ProjI8Tile pick_proj_i8_tile(int tokens, int channels, int steps, bool he
   float best = 0.f;
   ProjI8Tile tile = ProjI8Tile::kNone;
   for (const ProjI8Shape& s : kProjI8Shapes) {
-    if ((heads && channels / 3 % std::max(s.channels, 128) != 0) || (heads && s.channels < 128) ||
-        !proj_i8_fits(tokens, channels, s))
-      continue;
+    if ((heads && s.channels < 128) || !proj_i8_fits(tokens, channels, s)) continue;
     const float round = s.per_tile + s.per_step * (float)steps;
     // A round for each tile a CU gets at least: most shapes need no look at their lists.
     const int tiles_m = (int)(((int64_t)tokens + s.tokens - 1) / s.tokens);

@@ -43,7 +43,11 @@ SHAPES = [("256x256", 1000, 384, 40, 128), ("256x224", 801, 256, 40, 96),
           ("128x160", 257, 128, 40, 128), ("128x128", 129, 640, 40, 96),
           ("128x128p", 129, 128, 40, 128), ("128x64p", 65, 128, 40, 96),
           ("128x32p", 1, 128, 1, 96)]
-CASES = [s[1:] for s in SHAPES]
+# Odd head counts on tiles of 256 channels: the tiles between Q and K and between K and V
+# hold a head of each, the last one a single head.
+ODD_HEADS = [(900, 384, 39, 128), (2500, 256, 13, 96), (650, 384, 39, 96), (900, 256, 25, 128),
+             (385, 384, 41, 96), (4000, 256, 1, 128)]
+CASES = [s[1:] for s in SHAPES] + ODD_HEADS
 CASES += [(1, 128, 1, 128), (1, 5120, 40, 128), (5, 256, 3, 96), (16, 384, 2, 128),
          (17, 640, 2, 96), (33, 128, 5, 128), (65, 1152, 4, 96), (128, 256, 1, 96),
          (129, 512, 4, 128), (300, 1024, 7, 128), (637, 5120, 40, 128), (1151, 5376, 56, 96),
@@ -112,7 +116,7 @@ def test_fp32_rounding_against_64_bits(h3, S, K, H, rot):
 def test_more_padding_than_a_tile(h3):
     """seq_pad may lie far behind seq_len: every row between is zero, in all three parts."""
     from h3hip import ops
-    for S, K, H in ((3, 256, 3), (300, 384, 4), (1100, 640, 6)):
+    for S, K, H in ((3, 256, 3), (300, 384, 4), (1100, 640, 6), (900, 384, 39)):
         x, xs, w, ws = int8_operands(S, K, 3 * H * D, S)
         gq, gk = _gammas(2)
         table = _rope(S, 128, 1)[3]

@@ -1,6 +1,6 @@
 """The rule that picks an int8 projection's tile shape (csrc/proj_i8_tile.h, compiled here
 with g++): every size gets a shape that fits a launch and, for outputs written by heads, one
-that holds whole heads of one of Q, K and V; more rows or channels never make the picked
+that holds whole heads; more rows or channels never make the picked
 launch cheaper; and the shapes the GPU tests are meant to reach are reached."""
 import os
 import shutil
@@ -74,10 +74,10 @@ def test_every_tile_once_in_a_launch_that_fits(pick):
                                 (1, 2**31 - 1, 1, 0), (10_000_000, 1_000_000, 1, 0)])] == [0] * 4
 
 
-def test_heads_are_whole_and_of_one_part(pick):
+def test_heads_are_whole(pick):
     cases = [(t, 384 * h, k, 1) for t in TOKENS for h in (1, 2, 3, 5, 7, 40, 56) for k in (1, 8, 40)]
     for (t, n, k, _), (_, ch, _, once, _) in zip(cases, pick(cases)):
-        assert once and ch in (128, 256) and (n // 3) % ch == 0, (t, n, k, ch)
+        assert once and ch in (128, 256), (t, n, k, ch)
 
 
 def test_larger_calls_are_not_cheaper(pick):
@@ -98,3 +98,6 @@ def test_gpu_tests_reach_every_shape(pick):
     cases = [(S, N, K // 128, 0) for _, S, K, N in out.SHAPES]
     cases += [(S, 384 * H, K // 128, 1) for _, S, K, H, _ in qkv.SHAPES]
     assert [NAMES[int(c[0])] for c in pick(cases)] == NAMES + NAMES[:11]
+    # Odd head counts on tiles of two heads: both kinds of tile that hold two parts' or one head.
+    odd = pick([(S, 384 * H, K // 128, 1) for S, K, H, _ in qkv.ODD_HEADS])
+    assert [NAMES[int(c[0])] for c in odd[:5]] == NAMES[:5]
