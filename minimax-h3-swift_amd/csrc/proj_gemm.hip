@@ -22,11 +22,9 @@
 // same bits.
 //
 // Epilogue: the bf16 accumulators go to LDS as token rows (the rings are free
-// then), each wave takes whole rows of one head, 8 at a time in the prologue's
-// 8-lane layout, and normalises and rotates Q and K with the prologue's device
-// code (norm_rope.h) and the render's rotation table. Rows that are complete
-// run without a branch so that two passes overlap: one wave per SIMD has no
-// other to cover its latencies.
+// then), each wave takes whole rows, 8 at a time in the prologue's 8-lane layout, and
+// normalises and rotates Q and K with the prologue's device code (norm_rope.h) and
+// the render's rotation table (proj_rows.h, shared with the int8 projections).
 #include "gemm_loop.inc"
 #include "proj.h"
 #include "proj_rows.h"
