@@ -94,15 +94,15 @@ extern "C" int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scal
     return H3HIP_DECLINED;
   }
   const bool plain = q_gamma == nullptr && k_gamma == nullptr;
+  H3_REQUIRE(seq_len > 0 && heads > 0 && heads <= INT32_MAX / (3 * kHeadDim) &&
+                 seq_pad >= seq_len && seq_pad % 128 == 0,
+             H3HIP_EINVAL, "bad shape: seq_len %d seq_pad %d heads %d", seq_len, seq_pad, heads);
   const int rc = check_operands(x, ldx, x_scale, w, ldw, w_scale, hidden);
   if (rc != H3HIP_OK) return rc;
   H3_REQUIRE(q_out && k_out && v_out, H3HIP_EINVAL, "NULL tensor argument");
   H3_REQUIRE(plain || (q_gamma && k_gamma && rope_table), H3HIP_EINVAL,
              "gammas and the rotation table must all be given (or both gammas NULL for the "
              "plain GEMM)");
-  H3_REQUIRE(seq_len > 0 && heads > 0 && heads <= INT32_MAX / (3 * kHeadDim) &&
-                 seq_pad >= seq_len && seq_pad % 128 == 0,
-             H3HIP_EINVAL, "bad shape: seq_len %d seq_pad %d heads %d", seq_len, seq_pad, heads);
   H3_REQUIRE(rounding == H3HIP_ROUND_REFERENCE || rounding == H3HIP_ROUND_FP32, H3HIP_EINVAL,
              "unknown rounding mode %d", rounding);
   H3_REQUIRE(aligned(q_out, 16) && aligned(k_out, 16) && aligned(v_out, 16) &&

@@ -4,7 +4,8 @@
 //
 //   a = max_k |x[k]|,  q[k] = round_half_even(127 x[k] / a),  s = a / 127
 //
-// Bound by HBM: 2 bytes read and 1 written an element. A wave owns a row and
+// Bound by HBM: 2 bytes read and 1 written an element (31,885 x 5,120 in 92 us, 5.3 TB/s; a copy
+// of 2 GiB 4.9), of few rows by the launch (3.5 us). A wave owns a row and
 // holds it in registers between the maximum and the rounding (16 elements a lane
 // and chunk), so x is read once; rows of more than 8 chunks (8,192 elements) are
 // read twice, the second time from the caches.
@@ -16,6 +17,7 @@
 // it by at most 2^-19: it lands exactly on a tie that it stands for and cannot reach
 // one that it does not. Adding 1.5 * 2^23 then rounds half to even, and the sum's low
 // byte is q in two's complement.
+#include <algorithm>
 #include <climits>
 
 #include "common.h"
@@ -160,8 +162,11 @@ __global__ __launch_bounds__(64 * kWavesWg) void quant_rows_kernel(QuantArgs a) 
   }
 }
 
+// A launch takes fewer than 2^32 threads.
+constexpr int32_t kMaxRows = (1 << 30) / 64;
+
 void launch(const QuantArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.rows + (int64_t)kWavesWg - 1) / kWavesWg));
+  const dim3 grid((unsigned)((a.rows + kWavesWg - 1) / kWavesWg));
   const int chunks = (a.cols_pad + kChunk - 1) / kChunk;
   switch (chunks) {
 #define H3_CHUNKS(N) \
@@ -199,8 +204,10 @@ extern "C" int h3hip_quant_rows(const void* x, int64_t ldx, int32_t rows, int32_
                  (reinterpret_cast<uintptr_t>(q) & 15u) == 0 &&
                  (reinterpret_cast<uintptr_t>(scale) & 3u) == 0,
              H3HIP_EINVAL, "x must be 2-byte, q 16-byte and scale 4-byte aligned");
-  const QuantArgs a{static_cast<const uint16_t*>(x), static_cast<int8_t*>(q), scale, ldx, ldq,
-                    rows, cols, cols_pad};
-  launch(a, as_stream(stream));
+  for (int64_t m = 0; m < rows; m += kMaxRows)
+    launch(QuantArgs{static_cast<const uint16_t*>(x) + m * ldx, static_cast<int8_t*>(q) + m * ldq,
+                     scale + m, ldx, ldq, (int32_t)std::min<int64_t>(rows - m, kMaxRows), cols,
+                     cols_pad},
+           as_stream(stream));
   return check_launch("quant_rows_kernel");
 }

@@ -91,3 +91,18 @@ def test_rows_past_four_gigabytes(h3):
     _check(x[-3:], q[-3:], s[-3:])
     _check(x[:2], q[:2], s[:2])
     assert float(s[1:-3].abs().max()) == 0.0
+
+
+def test_more_rows_than_a_launch_takes(h3):
+    """2^24 + 5 rows of one element: the launch covers 2^24, the next one the rest."""
+    from h3hip import ops
+    S = (1 << 24) + 5
+    x = torch.zeros((S, 1), dtype=torch.bfloat16, device="cuda")
+    rows = [0, 1, (1 << 24) - 1, 1 << 24, S - 1]
+    x[rows, 0] = torch.tensor([1.0, -2.0, 3.0, -4.0, 5.0], dtype=torch.bfloat16, device="cuda")
+    note(f"quant_rows S={S}")
+    q, s = ops.quant_rows(x)
+    assert q[rows, 0].tolist() == [127, -127, 127, -127, 127] and not q[:, 1:].any()
+    assert int((s != 0).sum()) == 5 and int(q[:, 0].abs().sum()) == 5 * 127
+    want = torch.tensor([1.0, 2.0, 3.0, 4.0, 5.0]) / 127
+    assert torch.equal(s[rows].cpu(), want)

@@ -60,7 +60,7 @@ def test_proj_i8_declines(h3):
 
 
 @pytest.mark.parametrize("bad,word", [
-    (dict(k=0), "hidden"), (dict(S=0), "shape"), (dict(H=0), "shape"), (dict(pad=64), "shape"),
+    (dict(k=0), "hidden"), (dict(S=0), "shape"), (dict(S=0, pad=0, x=None), "shape"), (dict(H=0), "shape"), (dict(pad=64), "shape"),
     (dict(S=129), "shape"), (dict(H=6_000_000), "shape"), (dict(gq=None), "gammas"),
     (dict(table=None), "table"), (dict(rounding=2), "rounding"), (dict(q=None), "NULL"),
     (dict(v=ctypes.c_void_p(4104)), "aligned"), (dict(table=ctypes.c_void_p(4104)), "aligned"),
