@@ -4,11 +4,11 @@
 //
 //   a = max_k |x[k]|,  q[k] = round_half_even(127 x[k] / a),  s = a / 127
 //
-// Bound by HBM: 2 bytes read and 1 written an element (31,885 x 5,120 in 92 us, 5.3 TB/s; a copy
-// of 2 GiB 4.9), of few rows by the launch (3.5 us). A wave owns a row and
-// holds it in registers between the maximum and the rounding (16 elements a lane
-// and chunk), so x is read once; rows of more than 8 chunks (8,192 elements) are
-// read twice, the second time from the caches.
+// Bound by HBM: 2 bytes read and 1 written an element (31,885 x 5,120 in 88-92 us, 5.3-5.6 TB/s; a
+// copy of 2 GiB 4.9), of few rows by the launch (2.7 us). A row is held in the registers of the
+// wave or the workgroup that owns it between the maximum and the rounding (16 elements a
+// lane and chunk), so x is read once; rows of more than 16 chunks (16,384 elements) are read
+// twice, the second time from the caches.
 //
 // The quotient is never divided out. With i = 127 / a rounded to fp32, t = x i is
 // within 2^-23 (relative) of 127 x / a. x and a have 8-bit mantissas, so a quotient
@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kLaneElems = 16;                 // consecutive elements of a lane in a chunk
 constexpr int kChunk = 64 * kLaneElems;        // elements of a wave's chunk
-constexpr int kWavesWg = 4;                    // rows of a workgroup
+constexpr int kWavesWg = 4;                    // of a workgroup: a row each, or one shared
 constexpr uint32_t kAbs2 = 0x7fff7fffu;
 
 struct QuantArgs {
@@ -105,28 +105,31 @@ __device__ __forceinline__ void store_chunk(int8_t* row, int64_t k, int cols_pad
   *reinterpret_cast<u32x4*>(row + k) = o;
 }
 
-// kChunks: chunks of the row, held in registers; 0: any number, read twice.
-template <int kChunks>
+// kChunks: chunks of a wave's row, held in registers; 0: any number, read twice. kShared:
+// the workgroup's waves share a row, wave w taking its chunks w, w + kWavesWg, ...
+template <int kChunks, bool kShared>
 __global__ __launch_bounds__(64 * kWavesWg) void quant_rows_kernel(QuantArgs a) {
+  __shared__ uint32_t tops[kWavesWg];
   const int lane = threadIdx.x & 63;
-  const int64_t m = (int64_t)blockIdx.x * kWavesWg +
-                    __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int64_t m = kShared ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWavesWg + wave;
   if (m >= a.rows) return;
+  constexpr int kStride = kShared ? kWavesWg * kChunk : kChunk;   // from chunk to chunk of a wave
   const uint16_t* row = a.x + m * a.ldx;
   int8_t* out = a.q + m * a.ldq;
-  const int k0 = kLaneElems * lane;
+  const int k0 = kLaneElems * lane + (kShared ? kChunk * wave : 0);
   constexpr int kHeld = kChunks ? kChunks : 4;   // chunks in registers at once
   uint32_t v[kHeld][8];
   uint32_t top2 = 0;
   if constexpr (kChunks != 0) {
 #pragma unroll
-    for (int c = 0; c < kChunks; c++) load_chunk(row, k0 + c * kChunk, a.cols, v[c]);
+    for (int c = 0; c < kChunks; c++) load_chunk(row, k0 + c * kStride, a.cols, v[c]);
 #pragma unroll
     for (int c = 0; c < kChunks; c++) top2 = chunk_max(v[c], top2);
   } else {
-    for (int64_t k = 0; k < a.cols; k += kHeld * kChunk) {
+    for (int64_t k = k0; k < a.cols; k += kHeld * kStride) {
 #pragma unroll
-      for (int c = 0; c < kHeld; c++) load_chunk(row, k + k0 + c * kChunk, a.cols, v[c]);
+      for (int c = 0; c < kHeld; c++) load_chunk(row, k + c * kStride, a.cols, v[c]);
 #pragma unroll
       for (int c = 0; c < kHeld; c++) top2 = chunk_max(v[c], top2);
     }
@@ -134,6 +137,12 @@ __global__ __launch_bounds__(64 * kWavesWg) void quant_rows_kernel(QuantArgs a) 
   uint32_t top = max(top2 & 0xffffu, top2 >> 16);
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+  if constexpr (kShared) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWavesWg; w++) top = max(top, tops[w]);
+  }
   // A row that holds an infinity or a NaN has no int8 form: its scale is NaN, so
   // that whatever is multiplied with it shows, and its values are zeros.
   const bool finite = top < 0x7f80u;
@@ -143,45 +152,55 @@ __global__ __launch_bounds__(64 * kWavesWg) void quant_rows_kernel(QuantArgs a) 
     r.pre = amax < 0x1p-100f ? 0x1p100f : 1.f;
     r.inv = 127.0f / (amax * r.pre);
   }
-  if (lane == 0) a.scale[m] = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
+  if (lane == 0 && (!kShared || wave == 0))
+    a.scale[m] = finite ? amax / 127.0f : __uint_as_float(0x7fc00000u);
   if (!finite) {
-    for (int64_t k = k0; k < a.cols_pad; k += kChunk)
+    for (int64_t k = k0; k < a.cols_pad; k += kStride)
       *reinterpret_cast<u32x4*>(out + k) = u32x4{0u, 0u, 0u, 0u};
     return;
   }
   if constexpr (kChunks != 0) {
 #pragma unroll
-    for (int c = 0; c < kChunks; c++) store_chunk(out, k0 + c * kChunk, a.cols_pad, v[c], r);
+    for (int c = 0; c < kChunks; c++) store_chunk(out, k0 + c * kStride, a.cols_pad, v[c], r);
   } else {
-    for (int64_t k = 0; k < a.cols_pad; k += kHeld * kChunk) {
+    for (int64_t k = k0; k < a.cols_pad; k += kHeld * kStride) {
 #pragma unroll
-      for (int c = 0; c < kHeld; c++) load_chunk(row, k + k0 + c * kChunk, a.cols, v[c]);
+      for (int c = 0; c < kHeld; c++) load_chunk(row, k + c * kStride, a.cols, v[c]);
 #pragma unroll
-      for (int c = 0; c < kHeld; c++) store_chunk(out, k + k0 + c * kChunk, a.cols_pad, v[c], r);
+      for (int c = 0; c < kHeld; c++) store_chunk(out, k + c * kStride, a.cols_pad, v[c], r);
     }
   }
 }
 
 // A launch takes fewer than 2^32 threads.
-constexpr int32_t kMaxRows = (1 << 30) / 64;
+constexpr int32_t kMaxRows = (1 << 30) / (64 * kWavesWg);
+
+// A row a wave, or a row a workgroup. Shared, a row's latencies are a fourth each (one row of
+// 7,168 4.0 -> 2.8 us, 1,151 rows 8.8 -> 7.3), which is what few rows wait for; many rows need the
+// bytes in flight, and four waves with a chunk each hold fewer than four with a row each
+// (18,102 rows of 3,000 39 -> 42 us, of 2,048 17 -> 19). From two chunks a wave on sharing costs
+// nothing (31,885 x 5,120 90 -> 88 us, 18,102 x 6,000 62 -> 58, 4,000 x 12,000 41 -> 28).
+constexpr int kFewRows = 2048;
+
+template <bool kShared>
+void launch(const QuantArgs& a, int chunks, hipStream_t st) {
+  const dim3 grid((unsigned)(kShared ? a.rows : (a.rows + kWavesWg - 1) / kWavesWg));
+  const dim3 block(64 * kWavesWg);
+  switch (kShared ? (chunks + kWavesWg - 1) / kWavesWg : chunks) {
+    case 1: quant_rows_kernel<1, kShared><<<grid, block, 0, st>>>(a); break;
+    case 2: quant_rows_kernel<2, kShared><<<grid, block, 0, st>>>(a); break;
+    case 3: quant_rows_kernel<3, kShared><<<grid, block, 0, st>>>(a); break;
+    case 4: quant_rows_kernel<4, kShared><<<grid, block, 0, st>>>(a); break;
+    default: quant_rows_kernel<0, true><<<grid, block, 0, st>>>(a);   // shared
+  }
+}
 
 void launch(const QuantArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.rows + kWavesWg - 1) / kWavesWg));
   const int chunks = (a.cols_pad + kChunk - 1) / kChunk;
-  switch (chunks) {
-#define H3_CHUNKS(N) \
-  case N: quant_rows_kernel<N><<<grid, 64 * kWavesWg, 0, st>>>(a); break
-    H3_CHUNKS(1);
-    H3_CHUNKS(2);
-    H3_CHUNKS(3);
-    H3_CHUNKS(4);
-    H3_CHUNKS(5);
-    H3_CHUNKS(6);
-    H3_CHUNKS(7);
-    H3_CHUNKS(8);
-#undef H3_CHUNKS
-    default: quant_rows_kernel<0><<<grid, 64 * kWavesWg, 0, st>>>(a);
-  }
+  if (chunks > kWavesWg || (chunks > 2 && a.rows <= kFewRows))
+    launch<true>(a, chunks, st);
+  else
+    launch<false>(a, chunks, st);
 }
 
 }  // namespace

@@ -24,7 +24,9 @@ def _check(x, q, s):
 
 @pytest.mark.parametrize("S,K", [
     (1, 1), (1, 15), (3, 16), (17, 127), (1, 128), (20, 129), (4, 1000), (5, 1023), (6, 1024),
-    (7, 1025), (33, 2048), (18, 5120), (18, 5376), (3, 8191), (2, 8192), (3, 8193), (17, 20000),
+    (7, 1025), (33, 2048), (18, 2049), (18, 3073), (18, 4096), (18, 5120), (18, 5376), (3, 8191),
+    (2, 8192), (3, 8193), (17, 12288), (18, 12289), (17, 16384), (17, 16385), (17, 20000), (2049, 2500),
+    (2051, 3100), (2050, 4096), (2049, 4097), (2048, 2500),
     (1, 131072), (1000, 640)])
 def test_rows_exact(h3, S, K):
     from h3hip import ops
@@ -50,7 +52,7 @@ def test_rows_that_have_no_int8_form(h3):
     """An infinity or a NaN anywhere makes its row's scale NaN and its values 0, and
     no other row's."""
     from h3hip import ops
-    for K in (130, 5120, 9000):
+    for K in (130, 1500, 5120, 9000, 20000):
         x = rows_bf16(12, K, 5, special=False)
         x[1, 0], x[3, K - 1], x[5, K // 2] = float("inf"), float("-inf"), float("nan")
         note(f"quant_rows not finite K={K}")
