@@ -302,7 +302,7 @@ int h3hip_quant_rows(const void* x, int64_t ldx, int32_t rows, int32_t cols, voi
  *   x: device int8 [rows, in_features], row stride ldx bytes; w: device int8
  *      [out_features, in_features], row stride ldw bytes: as h3hip_quant_rows writes
  *      them (any values, -128 too; 16-byte aligned, strides multiples of 16).
- *   x_scale: device fp32 [rows]; w_scale: device fp32 [out_features], 16-byte aligned.
+ *   x_scale: device fp32 [rows]; w_scale: device fp32 [out_features].
  *   y: device bf16 [rows, out_features], row stride ldy elements; rows may begin
  *      anywhere, and nothing else is written.
  * Operands may pass 4 GiB; 256 rows of x or w must stay below 2 GiB.

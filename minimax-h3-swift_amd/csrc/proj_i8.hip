@@ -34,8 +34,8 @@ int check_operands(const void* x, int64_t ldx, const float* x_scale, const void*
   // A tile's rows are reached with 32-bit offsets from its first.
   H3_REQUIRE(ldx < kMaxStride && ldw < kMaxStride, H3HIP_EINVAL,
              "256 rows of x or w exceed 2 GiB (ldx %lld, ldw %lld)", (long long)ldx, (long long)ldw);
-  H3_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(x_scale, 4) && aligned(w_scale, 16),
-             H3HIP_EINVAL, "x, w and w_scale must be 16-byte aligned, x_scale 4-byte");
+  H3_REQUIRE(aligned(x, 16) && aligned(w, 16) && aligned(x_scale, 4) && aligned(w_scale, 4),
+             H3HIP_EINVAL, "x and w must be 16-byte aligned, their scales 4-byte");
   return H3HIP_OK;
 }
 

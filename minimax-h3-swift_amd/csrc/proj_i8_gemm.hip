@@ -28,6 +28,7 @@ constexpr int kWaves = H3_GEMM_I8_WAVES;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kStep = 128;               // reduction per step (bytes)
 
+typedef f32x4 f32x4_any __attribute__((aligned(4)));   // scales of any first channel
 typedef int i32x32 __attribute__((ext_vector_type(32)));
 // A wave's accumulators, 8 blocks of 16 x 16 to a vector (the last may be part used).
 template <int kNA, int kMB>
@@ -92,7 +93,7 @@ struct Scales {
     if (n0 + 32 * kNA <= a.n_total) {
 #pragma unroll
       for (int na = 0; na < kNA; na++)
-        w[na] = *reinterpret_cast<const f32x4*>(a.w_scale + n0 + 16 * (kNA * wc + na) + 4 * g);
+        w[na] = *reinterpret_cast<const f32x4_any*>(a.w_scale + n0 + 16 * (kNA * wc + na) + 4 * g);
       return;
     }
 #pragma unroll

@@ -129,6 +129,17 @@ def test_a_single_row_of_any_stride(h3):
     assert torch.equal(q, q2) and torch.equal(s, s2)
 
 
+@pytest.mark.parametrize("first,S,N", [(1, 3, 100), (3, 300, 517), (2, 700, 640), (5, 1500, 4000)])
+def test_some_rows_of_a_weight(h3, first, S, N):
+    """A weight's rows from any one on, with their scales: those channels' bits."""
+    from h3hip import ops
+    x, xs, w, ws = int8_operands(S, 256, N + 9, N)
+    note(f"proj_i8 channels {first}.. of {N + 9}, S={S}")
+    every = bits16(ops.proj_i8(x, xs, w, ws))
+    some = bits16(ops.proj_i8(x, xs, w[first:first + N], ws[first:first + N]))
+    assert (some == every[:, first:first + N]).all()
+
+
 def test_no_rows(h3):
     from h3hip import ops
     _, _, w, ws = int8_operands(1, 128, 40, 1)

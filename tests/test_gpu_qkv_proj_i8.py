@@ -113,6 +113,21 @@ def test_fp32_rounding_against_64_bits(h3, S, K, H, rot):
         assert worst <= 1.0
 
 
+@pytest.mark.parametrize("S,H", [(3, 2), (300, 3), (1000, 39)])
+def test_scales_at_any_address(h3, S, H):
+    from h3hip import ops
+    x, xs, w, ws = int8_operands(S, 256, 3 * H * D, S)
+    gq, gk = _gammas(4)
+    table = _rope(S, 96, 1)[3]
+    odd_x, odd_w = torch.zeros(S + 1, device="cuda")[1:], torch.zeros(3 * H * D + 3, device="cuda")[3:]
+    odd_x.copy_(xs), odd_w.copy_(ws)
+    note(f"qkv_proj_i8 scales at odd addresses S={S} H={H}")
+    want = ops.qkv_proj_i8(x, xs, w, ws, gq, gk, table, heads=H, rounding=1)
+    got = ops.qkv_proj_i8(x, odd_x, w, odd_w, gq, gk, table, heads=H, rounding=1)
+    for a, b in zip(got, want):
+        assert (bits16(a) == bits16(b)).all()
+
+
 def test_more_padding_than_a_tile(h3):
     """seq_pad may lie far behind seq_len: every row between is zero, in all three parts."""
     from h3hip import ops

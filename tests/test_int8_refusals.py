@@ -44,7 +44,7 @@ def test_no_rows_are_no_work(h3):
     (dict(ldx=264), "ldx"), (dict(ldw=128), "ldw"), (dict(ldy=63), "ldy"), (dict(x=None), "NULL"),
     (dict(xs=None), "NULL"), (dict(w=None), "NULL"), (dict(ws=None), "NULL"), (dict(y=None), "NULL"),
     (dict(x=ctypes.c_void_p(4104)), "aligned"), (dict(w=ctypes.c_void_p(4104)), "aligned"),
-    (dict(ws=ctypes.c_void_p(4100)), "aligned"), (dict(xs=ctypes.c_void_p(4098)), "aligned"),
+    (dict(ws=ctypes.c_void_p(4098)), "aligned"), (dict(xs=ctypes.c_void_p(4098)), "aligned"),
     (dict(y=ctypes.c_void_p(4097)), "aligned"), (dict(ldx=1 << 26), "2 GiB"),
     (dict(ldw=1 << 26), "2 GiB")])
 def test_proj_i8(h3, bad, word):
