@@ -42,6 +42,14 @@ __device__ __forceinline__ void zero_rows(const ProjArgs& a, int tid, int m0, in
   }
 }
 
+// Between a wave's LDS accesses that meet in other lanes: the hardware runs them in order, and
+// this keeps the compiler from changing it. No instruction.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // The rotation entries of 8 token rows, from the table to the lanes of the prologue's
 // row layout: lane j of row group rg needs entries 8j .. 8j + 7 of its row, 128 bytes
 // (fp32; 64 in bf16) from its neighbour's. Loaded like that every load of a wave touches
@@ -78,6 +86,7 @@ struct RowTable {
   // From the loaded registers to tab, through the wave's lds; the pairs of pair lanes.
   __device__ __forceinline__ void trade(RopeEntry* lds, int j, int rg, RopeEntry (&tab)[8]) {
     RopeEntry* mine = lds + 64 * rg;
+    wave_lds_order();   // the last pass's reads
 #pragma unroll
     for (int t = 0; t < kLoads; t++) {
       if constexpr (kRef) {   // entries 16t + 2j, + 1: (c, -s, s, c) bf16 each
@@ -90,6 +99,7 @@ struct RowTable {
         *reinterpret_cast<f32x2*>(mine + 8 * (t ^ rg) + 2 * ((j >> 1) ^ unit(t, rg)) + (j & 1)) = v;
       }
     }
+    wave_lds_order();
 #pragma unroll
     for (int q = 0; q < 4; q++) {
       const f32x4 v = *reinterpret_cast<const f32x4*>(mine + 8 * (j ^ rg) + 2 * (q ^ unit(j, rg)));
