@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Writes gemm_i8_loop.inc: the reduction loops of the int8 projections
-(proj_i8_gemm.hip) as gfx950 inline assembly, one block per tile shape.
+(proj_i8_kernel.h) as gfx950 inline assembly, one block per tile shape.
 
 The stream is gen_gemm_loop.py's. A step's rows are 128 bytes there as here, 128
 int8 values in place of 64 bf16 ones, and v_mfma_i32_16x16x64_i8 takes 16 bytes of

@@ -1,4 +1,4 @@
-// Arguments of the int8 projections' kernel (proj_i8_gemm.hip) and its launch.
+// Arguments of the int8 projections' kernel (proj_i8_kernel.h) and its launch.
 #pragma once
 
 #include "proj.h"

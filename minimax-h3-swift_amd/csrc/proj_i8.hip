@@ -1,4 +1,4 @@
-// The int8 projections' entry points (kernel: proj_i8_gemm.hip).
+// The int8 projections' entry points (kernel: proj_i8_kernel.h).
 //
 //   y[m, n] = ((sum_k x[m, k] w[n, k]) w_scale[n]) x_scale[m]
 //

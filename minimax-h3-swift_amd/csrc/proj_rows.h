@@ -1,7 +1,7 @@
 // The second half of a projection's epilogue: the bf16 product, staged in LDS as
-// token rows, to the outputs, with the head norm and the rotation on the way.
-// Shared by the bf16 and the int8 projections (proj_gemm.hip, proj_i8.hip,
-// proj_i8_gemm.hip), whose accumulators differ and whose rows do not.
+// token rows, to the outputs, with the head norm and the rotation on the way. Shared by
+// the bf16 and the int8 projections (proj_gemm.hip, proj_i8_kernel.h), whose accumulators
+// differ and whose rows do not.
 #pragma once
 
 #include <type_traits>
