@@ -56,6 +56,10 @@ extern "C" {
 #define H3HIP_ROUND_REFERENCE 0 /* bf16 after RMSNorm and after every RoPE product and sum,
                                    as MLX does on bf16 arrays (DiTBlock.swift:83-103) */
 #define H3HIP_ROUND_FP32 1      /* fp32 until the single store */
+#define H3HIP_ROUND_ONCE 3      /* FP32, and the projection's product stays fp32 as well, where
+                                   FP32 normalises the bf16 product: one rounding to bf16 from
+                                   the operands to Q and K. h3hip_qkv_proj_i8 only;
+                                   h3hip_rope_table writes FP32's table for it */
 
 /* Output layouts of the attention. */
 #define H3HIP_OUT_HEAD_MAJOR 0  /* [heads, seq_pad, head_dim] */
@@ -233,7 +237,7 @@ int h3hip_head_major(const void* in, int64_t ld_in, int32_t seq_len, int32_t seq
  *   pos, pair_axis, pair_inv_freq, rot: as for h3hip_qk_norm_rope.
  *   table: device [seq_len, rot/2, 2, 2] holding [[c, -s], [s, c]] per token and
  *          pair: bf16 for H3HIP_ROUND_REFERENCE (the reference's bf16 table),
- *          fp32 for H3HIP_ROUND_FP32; 16-byte aligned.
+ *          fp32 for H3HIP_ROUND_FP32 and H3HIP_ROUND_ONCE; 16-byte aligned.
  * The entries are the ones h3hip_qk_norm_rope rotates with. */
 int h3hip_rope_table(const float* pos, const int32_t* pair_axis, const float* pair_inv_freq,
                      int32_t rot, int32_t rounding, int32_t seq_len, void* table, void* stream);
@@ -315,7 +319,8 @@ int h3hip_proj_i8(const void* x, int64_t ldx, const float* x_scale, const void* 
 /* h3hip_qkv_proj on int8 operands: the product of h3hip_proj_i8 for Q | K | V rows of
  * w, rounded to bf16, with the head norm and the rotation in its epilogue. Q and K come
  * out equal, bit for bit, to h3hip_qk_norm_rope applied to h3hip_proj_i8's result; V is
- * that result, head-major.
+ * that result, head-major. With H3HIP_ROUND_ONCE Q and K are the norm and the rotation of the
+ * fp32 product instead, rounded to bf16 only when they are stored; V is the same.
  *   x, x_scale, w, w_scale: as for h3hip_proj_i8, w [3*heads*head_dim, hidden].
  *   Everything else as for h3hip_qkv_proj (both gammas NULL: the plain product, head-major).
  * Declines unless head_dim == 128, rot is 96 or 128 and hidden is a multiple of 128 of

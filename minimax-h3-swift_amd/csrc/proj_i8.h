@@ -2,6 +2,7 @@
 #pragma once
 
 #include "proj.h"
+#include "proj_i8_tile.h"
 
 namespace h3hip {
 
@@ -20,5 +21,7 @@ struct ProjI8Args {
 // Launches proj_i8_gemm_kernel on the tile shape that suits the sizes (proj_i8_gemm.hip).
 int launch_proj_i8_gemm(const ProjI8Args& a, int32_t rounding, bool plain, bool out,
                         hipStream_t stream);
+// The same for Q | K | V in H3HIP_ROUND_ONCE, on a given shape (proj_i8_once.hip).
+int launch_proj_i8_once(const ProjI8Args& a, ProjI8Tile tile, hipStream_t stream);
 
 }  // namespace h3hip

@@ -103,8 +103,9 @@ extern "C" int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scal
   H3_REQUIRE(plain || (q_gamma && k_gamma && rope_table), H3HIP_EINVAL,
              "gammas and the rotation table must all be given (or both gammas NULL for the "
              "plain GEMM)");
-  H3_REQUIRE(rounding == H3HIP_ROUND_REFERENCE || rounding == H3HIP_ROUND_FP32, H3HIP_EINVAL,
-             "unknown rounding mode %d", rounding);
+  H3_REQUIRE(rounding == H3HIP_ROUND_REFERENCE || rounding == H3HIP_ROUND_FP32 ||
+                 rounding == H3HIP_ROUND_ONCE,
+             H3HIP_EINVAL, "unknown rounding mode %d", rounding);
   H3_REQUIRE(aligned(q_out, 16) && aligned(k_out, 16) && aligned(v_out, 16) &&
                  (plain || (aligned(rope_table, 16) && aligned(q_gamma, 16) && aligned(k_gamma, 16))),
              H3HIP_EINVAL, "tensors must be 16-byte aligned");

@@ -1,6 +1,6 @@
 // Launches of the int8 projections' kernel (proj_i8_kernel.h): a tile shape by size
 // (proj_i8_tile.h), in the forms of the out-projection, the plain QKV product and the QKV
-// product with norm and rotation.
+// product with norm and rotation in two roundings (the third: proj_i8_once.hip).
 #include "proj_i8_kernel.h"
 
 namespace h3hip {
@@ -9,10 +9,7 @@ namespace {
 
 template <int kNA, int kMB, bool kPair>
 int launch(ProjI8Args a, int32_t rounding, bool plain, bool out, hipStream_t st) {
-  const ProjGrid g = proj_i8_grid(a.out.seq_len, a.n_total, 32 * kMB, 32 * kNA);
-  a.out.tiles_m = g.order.tiles_m;
-  a.out.chunk = g.order.chunk;
-  const dim3 grid(kOrderXcds * g.longest);
+  const dim3 grid = order_grid<kNA, kMB>(a);
   constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32;
   if (out) {
     proj_i8_gemm_kernel<kNA, kMB, kPair, kRef, 8, true, true><<<grid, kThreads, 0, st>>>(a);
@@ -35,7 +32,9 @@ int launch(ProjI8Args a, int32_t rounding, bool plain, bool out, hipStream_t st)
 
 int launch_proj_i8_gemm(const ProjI8Args& a, int32_t rounding, bool plain, bool out,
                         hipStream_t stream) {
-  switch (pick_proj_i8_tile(a.out.seq_len, a.n_total, a.in / kStep, !out)) {
+  const ProjI8Tile tile = pick_proj_i8_tile(a.out.seq_len, a.n_total, a.in / kStep, !out);
+  if (rounding == H3HIP_ROUND_ONCE && !plain) return launch_proj_i8_once(a, tile, stream);
+  switch (tile) {
     case ProjI8Tile::k256x256: return launch<8, 8, false>(a, rounding, plain, out, stream);
     case ProjI8Tile::k256x224: return launch<8, 7, false>(a, rounding, plain, out, stream);
     case ProjI8Tile::k256x192: return launch<8, 6, false>(a, rounding, plain, out, stream);
@@ -52,8 +51,7 @@ int launch_proj_i8_gemm(const ProjI8Args& a, int32_t rounding, bool plain, bool 
     case ProjI8Tile::k32x32p: return launch<1, 1, true>(a, rounding, plain, out, stream);
     default: break;
   }
-  set_error("too many rows or channels for one launch (%d x %d)", a.out.seq_len, a.n_total);
-  return H3HIP_EINVAL;
+  return too_large(a);
 }
 
 }  // namespace h3hip

@@ -44,8 +44,9 @@ extern "C" int h3hip_rope_table(const float* pos, const int32_t* pair_axis,
   H3_REQUIRE(pos && pair_axis && pair_inv_freq && table, H3HIP_EINVAL, "NULL argument");
   H3_REQUIRE(rot > 0 && rot % 2 == 0 && seq_len > 0, H3HIP_EINVAL, "bad rot %d / seq_len %d",
              rot, seq_len);
-  H3_REQUIRE(rounding == H3HIP_ROUND_REFERENCE || rounding == H3HIP_ROUND_FP32, H3HIP_EINVAL,
-             "unknown rounding mode %d", rounding);
+  H3_REQUIRE(rounding == H3HIP_ROUND_REFERENCE || rounding == H3HIP_ROUND_FP32 ||
+                 rounding == H3HIP_ROUND_ONCE,
+             H3HIP_EINVAL, "unknown rounding mode %d", rounding);
   H3_REQUIRE((reinterpret_cast<uintptr_t>(table) & 15u) == 0, H3HIP_EINVAL,
              "table must be 16-byte aligned");
   const int32_t half = rot / 2;

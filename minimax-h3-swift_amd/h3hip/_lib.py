@@ -17,7 +17,7 @@ EINVAL, EHIP, ENOMEM, EDEVICE = -1, -2, -3, -4
 TILE = 128
 
 RULE_DENSE, RULE_BAND, RULE_LOCAL, RULE_AXIAL, RULE_BITMAP = 0, 1, 2, 3, 4
-ROUND_REFERENCE, ROUND_FP32 = 0, 1
+ROUND_REFERENCE, ROUND_FP32, ROUND_ONCE = 0, 1, 3
 OUT_HEAD_MAJOR, OUT_TOKEN_MAJOR = 0, 1
 
 _i32p = ctypes.POINTER(ctypes.c_int32)

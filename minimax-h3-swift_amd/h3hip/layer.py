@@ -19,7 +19,8 @@ the stages.
 
 With ``projection="int8"`` both projections run on int8 operands with scales for
 each token and output channel (h3hip_quant_rows, h3hip_qkv_proj_i8,
-h3hip_proj_i8): the weights are rounded once, the activations in every call.
+h3hip_proj_i8): the weights are rounded once, the activations in every call. A
+RopeState of ROUND_ONCE keeps Q and K in fp32 from that product to their store.
 """
 from __future__ import annotations
 
@@ -174,6 +175,8 @@ class AttentionLayer:
             raise ValueError(f"x must be [S, {self.qkv_weight.shape[1]}] (the packed-row layout), "
                              f"got {tuple(x.shape)}")
         S = x.shape[0]
+        if rope is not None and rope.rounding == L.ROUND_ONCE and self.projection != "int8":
+            raise ValueError("ROUND_ONCE needs projection='int8'")
         if rope is None:
             rope = RopeState.identity(S, self.head_dim, x.device)
         seq_pad = ((S + L.TILE - 1) // L.TILE) * L.TILE

@@ -160,7 +160,7 @@ def rope_table(pos: torch.Tensor, pair_axis: torch.Tensor, pair_inv: torch.Tenso
                rot: int | None = None, rounding: int = L.ROUND_REFERENCE,
                out: torch.Tensor | None = None) -> torch.Tensor:
     """The render's rotation table (H3RoPE.rotationTable): [S, rot/2, 2, 2]
-    holding [[c, -s], [s, c]], bf16 for REFERENCE rounding, fp32 for FP32."""
+    holding [[c, -s], [s, c]], bf16 for REFERENCE rounding, fp32 for FP32 and ONCE."""
     for name, t, dt in (("pos", pos, torch.float32), ("pair_axis", pair_axis, torch.int32),
                         ("pair_inv", pair_inv, torch.float32)):
         if not t.is_cuda or t.dtype != dt or not t.is_contiguous():
@@ -385,8 +385,9 @@ def qkv_proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
                 rounding: int = L.ROUND_REFERENCE, out=None):
     """qkv_proj() on int8 operands (x, x_scale, w, w_scale as for proj_i8(), w
     [3*heads*head_dim, hidden]): the QKV product with the Q/K norm + RoPE in its
-    epilogue. Returns (q, k, v) as [heads, seq_pad, head_dim] bf16, or None when the
-    geometry is declined."""
+    epilogue. ROUND_REFERENCE and ROUND_FP32 normalise the bf16 product, as qkv_proj()
+    does; ROUND_ONCE keeps it in fp32 up to the one rounding of Q and K. Returns (q, k, v)
+    as [heads, seq_pad, head_dim] bf16, or None when the geometry is declined."""
     device, S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
     if N != 3 * heads * head_dim:
         raise ValueError(f"w must be [{3 * heads * head_dim}, {K}], got {tuple(w.shape)}")
