@@ -202,7 +202,7 @@ def run(state):
     if c["op"] == "linear":
         return ops.proj_i8(q, s, state["wq"], state["t"])
     return ops.qkv_proj_i8(q, s, state["wq"], state["t"], *state["gammas"], state["table"],
-                           heads=c["heads"], eps=EPS, rounding=L.ROUND_FP32)
+                           heads=c["heads"], eps=EPS, rounding=L.ROUND_ONCE)
 
 
 def _framework():
