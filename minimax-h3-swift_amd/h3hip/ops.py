@@ -278,6 +278,15 @@ def _run(fn, device: torch.device, *args) -> int:
     return rc if rc == L.OK else L.check(rc, allow_declined=True)
 
 
+# Sizes go to 32-bit parameters, into which ctypes cuts a larger number without an error.
+_INT32_MAX = 2 ** 31 - 1
+
+
+def _require_int32(name: str, t: torch.Tensor):
+    if max(t.shape) > _INT32_MAX:
+        raise ValueError(f"{name} must have sizes below 2^31, got {tuple(t.shape)}")
+
+
 def _require_same_device(device: torch.device, **others):
     for name, t in others.items():
         if t.device != device:
@@ -315,6 +324,7 @@ def quant_rows(x: torch.Tensor, out=None):
     S, K = x.shape
     if K == 0:
         raise ValueError("x must be [S, K > 0]")
+    _require_int32("x", x)
     if not x.is_cuda:
         raise ValueError("x must be a GPU tensor (no host fallback exists)")
     device, pad = x.device, (K + 127) // 128 * 128
@@ -338,6 +348,9 @@ def _int8_operands(x, x_scale, w, w_scale):
     """Checks the operands of an int8 projection; returns (device, S, K, N, ldx, ldw)."""
     if x.dim() == w.dim() == 2:
         (S, K), (N, k) = x.shape, w.shape
+        if S > _INT32_MAX or K > _INT32_MAX or N > _INT32_MAX:
+            _require_int32("x", x)
+            _require_int32("w", w)
         (ldx, step), (ldw, step_w) = x.stride(), w.stride()
         device = x.device
         if (x.dtype is _I8 and w.dtype is _I8 and x_scale.dtype is _F32 and w_scale.dtype is _F32
