@@ -94,7 +94,8 @@ class AttentionLayer:
     or "hipblaslt" (GEMM + h3hip_qk_norm_rope); either falls back to the other
     when its kernel declines the geometry. "int8" runs both projections on int8
     operands (qkv_weight and out_weight are rounded here, or given as Int8Weight;
-    the bf16 ones are not kept, so nothing is fallen back to)."""
+    the bf16 ones are not kept, so nothing is fallen back to), of at most
+    ops.INT8_MAX_REDUCTION in features, padded to a multiple of 128."""
 
     def __init__(self, qkv_weight, out_weight, q_gamma, k_gamma, *, heads: int,
                  head_dim: int = 128, eps: float = 1e-5, backend: H3AttentionBackend | None = None,
@@ -106,6 +107,11 @@ class AttentionLayer:
         if qkv_weight.shape[0] != 3 * inner or out_weight.shape[1] != inner:
             raise ValueError("weights do not match heads * head_dim")
         if projection == "int8":
+            for name, w in (("qkv_weight", qkv_weight), ("out_weight", out_weight)):
+                if (w.shape[1] + 127) // 128 * 128 > ops.INT8_MAX_REDUCTION:
+                    raise NotImplementedError(
+                        f"no int8 kernel takes {name}'s {w.shape[1]} in features (at most "
+                        f"{ops.INT8_MAX_REDUCTION}, padded to a multiple of 128)")
             qkv_weight, out_weight = (w if isinstance(w, Int8Weight) else Int8Weight.round(w)
                                       for w in (qkv_weight, out_weight))
         elif isinstance(qkv_weight, Int8Weight) or isinstance(out_weight, Int8Weight):

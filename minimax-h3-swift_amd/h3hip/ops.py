@@ -262,6 +262,7 @@ def out_proj(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None):
 # small: the raw stream handle without a Stream object, the device switched only where the
 # operands are not on the current one, sizes given to torch.empty one by one (1.3 us; as a
 # tuple 1.7).
+INT8_MAX_REDUCTION = 131071      # in features whose sums stay in int32, whatever the values
 _I8, _F32, _BF16 = torch.int8, torch.float32, torch.bfloat16
 _empty = torch.empty
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
