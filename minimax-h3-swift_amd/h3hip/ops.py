@@ -265,17 +265,16 @@ def out_proj(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None):
 INT8_MAX_REDUCTION = 131071      # in features whose sums stay in int32, whatever the values
 _I8, _F32, _BF16 = torch.int8, torch.float32, torch.bfloat16
 _empty = torch.empty
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _run(fn, device: torch.device, *args) -> int:
     """fn(*args, stream) on the current stream of ``device``; DECLINED or OK."""
-    index = device.index
-    if _current_device() == index:
-        rc = fn(*args, _raw_stream(index))
+    index, gpu = device.index, torch._C     # a torch without a GPU backend has neither function
+    if gpu._cuda_getDevice() == index:
+        rc = fn(*args, gpu._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(*args, gpu._cuda_getCurrentRawStream(index))
     return rc if rc == L.OK else L.check(rc, allow_declined=True)
 
 
