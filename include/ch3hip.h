@@ -302,7 +302,8 @@ int h3hip_quant_rows(const void* x, int64_t ldx, int32_t rows, int32_t cols, voi
  *   y[m, n] = ((sum_k x[m, k] w[n, k]) * w_scale[n]) * x_scale[m]
  * The sum is exact (int32); it, and its products with the scales, are rounded to
  * fp32, the result once to bf16. The int8 form of h3hip_out_proj, for any number of
- * rows (0 and 1 too) and any width.
+ * rows (0 and 1 too) and any width up to 16,776,960 of either and 2^23 tiles of 256 x 256
+ * (H3HIP_EINVAL past them).
  *   x: device int8 [rows, in_features], row stride ldx bytes; w: device int8
  *      [out_features, in_features], row stride ldw bytes: as h3hip_quant_rows writes
  *      them (any values, -128 too; 16-byte aligned, strides multiples of 16).
@@ -324,7 +325,8 @@ int h3hip_proj_i8(const void* x, int64_t ldx, const float* x_scale, const void* 
  *   x, x_scale, w, w_scale: as for h3hip_proj_i8, w [3*heads*head_dim, hidden].
  *   Everything else as for h3hip_qkv_proj (both gammas NULL: the plain product, head-major).
  * Declines unless head_dim == 128, rot is 96 or 128 and hidden is a multiple of 128 of
- * at most 131,071; any head count. */
+ * at most 131,071; any head count. seq_len and 3*heads*128 are limited as rows and width
+ * are for h3hip_proj_i8. */
 int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
                       const float* w_scale, int32_t hidden, const void* q_gamma,
                       const void* k_gamma, float eps, const void* rope_table, int32_t rot,

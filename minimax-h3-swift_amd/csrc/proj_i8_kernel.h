@@ -1,4 +1,4 @@
-// The int8 projections' GEMM on four waves: tiles of W x^T, from one row to any number.
+// The int8 projections' GEMM on four waves: tiles of W x^T, from one row up.
 //
 // The loop is the bf16 GEMM's (proj_gemm.hip has its layout and why it is four waves)
 // with v_mfma_i32_16x16x64_i8 in place of the bf16 product: twice the operations for the

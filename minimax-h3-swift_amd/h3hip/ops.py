@@ -375,7 +375,7 @@ def proj_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     """A projection on int8 operands: y = (x . w^T) * w_scale * x_scale[:, None].
 
     x: [S, K] int8 and x_scale: [S] fp32, w: [N, K] int8 and w_scale: [N] fp32, as
-    quant_rows() makes them (K a multiple of 128). Returns y [S, N] bf16 (or writes
+    quant_rows() makes them (K a multiple of 128; S and N up to 16,776,960). Returns y [S, N] bf16 (or writes
     ``out``, any row stride), or None when declined."""
     device, S, K, N, ldx, ldw = _int8_operands(x, x_scale, w, w_scale)
     if out is None:
