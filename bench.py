@@ -602,7 +602,8 @@ def attention_layer_extra(args, env):
     h3hip_out_proj); the fused projection with hipBLASLt's out-projection
     (torch.mm); and hipBLASLt's GEMMs with the prologue kernel between them
     (V then read in place from the token-major qkv). The out-projection alone
-    is timed both ways beside them."""
+    is timed both ways beside them. Then the first path in turn with the same layer on
+    int8 projections (weights rounded before, activations in the timed call)."""
     import numpy as np
     import torch
     from h3hip import ops
@@ -667,6 +668,25 @@ def attention_layer_extra(args, env):
     res["layer_tflop"] = round(flops / 1e12, 4)
     best = min(res["all_h3hip_ms"], res["fused_qkv_ms"], res["hipblaslt_qkv_ms"])
     res["best_tflops"] = round(flops / (best * 1e-3) / 1e12, 1)
+
+    w8, w8_out = ops.quant_rows(w), ops.quant_rows(w_out)
+    x8, att8 = (tuple(torch.empty_like(t) for t in ops.quant_rows(a)) for a in (x, att))
+    y8 = torch.empty_like(y)
+
+    def int8_path():
+        ops.quant_rows(x, out=x8)
+        ops.qkv_proj_i8(*x8, *w8, env["gq"], env["gk"], table, heads=H, eps=eps, seq_pad=S_pad,
+                        out=(qh, kh, vh))
+        ops.bsattn_fwd_strided(plan, qh, kh, vh, scale, out=att_view)
+        ops.quant_rows(att, out=att8)
+        ops.proj_i8(*att8, *w8_out, out=y8)
+
+    med = interleaved_medians({"bf16": all_h3hip_path, "int8": int8_path},
+                              reps=max(12, args.steps))
+    rel = float((y8.double() - y.double()).norm() / y.double().norm())
+    res["int8_projections"] = {"timing": "medians of interleaved calls",
+                               "int8_ms": round(med["int8"], 4), "bf16_ms": round(med["bf16"], 4),
+                               "rel_rms_vs_bf16": round(rel, 5)}
     return res
 
 
