@@ -7,9 +7,10 @@
 // a tile at either edge needs no case of its own before its stores.
 //
 // What bounds it: large products the chip's power limit (31,885 x 5,120 x 15,360 on random
-// operands 1.86 ms, 2,690 TOP/s, on zeros 1.39), the library's int8 product of these sizes takes
-// 2.13; few rows W's bytes (one token x 5,120 x 15,360 with norm 16-19 us, 4.6-5.2 TB/s) and, of a
-// small W, the launch and 40 steps' latencies (one token x 5,120 x 5,120 7.1 us, 125 tokens 11.7).
+// operands 1.86 ms, 2,690 TOP/s, on zeros 1.39; the library's int8 product of these sizes takes
+// 2.07-2.13); few rows W's bytes (one token x 5,120 x 15,360 with norm 16.3-17.5 us, 4.5-4.8 TB/s
+// with the launch) and, of a small W, the launch and 40 steps' latencies (one token x 5,120 x
+// 5,120 7.1 us, 125 tokens 11.8).
 //
 // Epilogue: each sum to fp32, times its channel's and its token's scale, to bf16, into
 // LDS as token rows, and from there what the bf16 projections do (proj_rows.h); in

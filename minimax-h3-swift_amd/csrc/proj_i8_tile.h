@@ -72,7 +72,9 @@ inline ProjGrid proj_i8_grid(int tokens, int channels, int tile_tokens, int tile
 // The constants are least squares over 440 sizes (1 to 18,102 tokens, 777 to 15,360
 // channels, 3 to 56 steps, without norm) of every shape on MI355X, whose times they give to
 // 9-19% (rms). What they pick is within 0.9% of the fastest shape on average, 15% at most, and
-// within 1.4-2.4% (31%) on 1,074 sizes of the QKV forms, which they were not fitted to. Few
+// within 1.4-2.4% (31%) on 1,074 sizes of the QKV forms, which they were not fitted to. They
+// rank shapes and are no time of a call: neither the norm nor W's bytes are in them (QKV of
+// 1,151 x 56 heads x 5,376 is 89 us by them and takes 116-120). Few
 // rows are where it matters: one token x 5,120 x 5,120 takes 7.5 us on 160 tiles of 32 x 32,
 // 15.7 on 40 of 128 x 64 and 27 on 20 of 256 x 128; 125 tokens 12.7 on 64 x 64, 15.4 on 32 x 32.
 inline ProjI8Tile pick_proj_i8_tile(int tokens, int channels, int steps, bool heads) {
