@@ -8,7 +8,7 @@
 // h3hip_qkv_proj_i8 treats it as Q | K | V heads and ends as h3hip_qkv_proj does, with
 // the bf16 product normalised and rotated by the code of the bf16 path
 // (proj_rows.h), so its Q and K are h3hip_qk_norm_rope of h3hip_proj_i8's result, bit
-// for bit.
+// for bit; in H3HIP_ROUND_ONCE the fp32 product is, and rounded at the store.
 #include "proj_i8.h"
 
 namespace h3hip {

@@ -239,9 +239,9 @@ __device__ __forceinline__ void finish_tile_once(const ProjI8Args& a, float* lds
     };
     if (one_part) {
       finish_heads(0, std::integral_constant<int, kHeads>{});
-    } else {
+    } else {   // the last head of Q or K and the first of the part behind it
 #pragma unroll 1
-      for (int nh = 0; nh < 2 && hg0 + nh < 3 * o.heads; nh++)
+      for (int nh = 0; nh < 2; nh++)
         finish_heads(nh, std::integral_constant<int, 1>{});
     }
   }
