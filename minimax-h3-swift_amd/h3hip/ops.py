@@ -265,16 +265,19 @@ def out_proj(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None):
 INT8_MAX_REDUCTION = 131071      # in features whose sums stay in int32, whatever the values
 _I8, _F32, _BF16 = torch.int8, torch.float32, torch.bfloat16
 _empty = torch.empty
+# A torch built without a GPU backend has neither function (and no tensor that needs them).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _run(fn, device: torch.device, *args) -> int:
     """fn(*args, stream) on the current stream of ``device``; DECLINED or OK."""
-    index, gpu = device.index, torch._C     # a torch without a GPU backend has neither function
-    if gpu._cuda_getDevice() == index:
-        rc = fn(*args, gpu._cuda_getCurrentRawStream(index))
+    index = device.index
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, gpu._cuda_getCurrentRawStream(index))
+            rc = fn(*args, _raw_stream(index))
     return rc if rc == L.OK else L.check(rc, allow_declined=True)
 
 
@@ -324,7 +327,8 @@ def quant_rows(x: torch.Tensor, out=None):
     S, K = x.shape
     if K == 0:
         raise ValueError("x must be [S, K > 0]")
-    _require_int32("x", x)
+    if S > _INT32_MAX or K > _INT32_MAX:
+        _require_int32("x", x)
     if not x.is_cuda:
         raise ValueError("x must be a GPU tensor (no host fallback exists)")
     device, pad = x.device, (K + 127) // 128 * 128
