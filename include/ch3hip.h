@@ -58,8 +58,9 @@ extern "C" {
 #define H3HIP_ROUND_FP32 1      /* fp32 until the single store */
 #define H3HIP_ROUND_ONCE 3      /* FP32, and the projection's product stays fp32 as well, where
                                    FP32 normalises the bf16 product: one rounding to bf16 from
-                                   the operands to Q and K. h3hip_qkv_proj_i8 only;
-                                   h3hip_rope_table writes FP32's table for it */
+                                   the operands to Q and K. h3hip_qkv_proj_i8 and
+                                   h3hip_qkv_proj_mx4 only; h3hip_rope_table writes FP32's
+                                   table for it */
 
 /* Output layouts of the attention. */
 #define H3HIP_OUT_HEAD_MAJOR 0  /* [heads, seq_pad, head_dim] */
@@ -332,6 +333,66 @@ int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scale, const vo
                       const void* k_gamma, float eps, const void* rope_table, int32_t rot,
                       int32_t rounding, int32_t seq_len, int32_t seq_pad, int32_t heads,
                       int32_t head_dim, void* q_out, void* k_out, void* v_out, void* stream);
+
+/* ------------------------------------------- microscaled 4-bit projections */
+
+/* Rows of bf16 rounded to 4-bit floats with a power of two for every 32 consecutive values
+ * (MXFP4 of the OCP Microscaling Formats specification, v1.0), the operands of the 4-bit
+ * projections: activations on every call, weights once. No counterpart in the reference,
+ * whose projections are bf16 matmuls (DiTBlock.swift:336-359).
+ *   a = max |x| of a block, e = max(floor(log2 a) - 2, -127), q = x / 2^e rounded to
+ *   0, 0.5, 1, 1.5, 2, 3, 4 or 6 with x's sign, half to the even code, at most 6. Every
+ *   step but q's rounding is exact. A block that holds an infinity or a NaN has the scale
+ *   NaN and values 0: every product with it is NaN.
+ *   x:     device bf16 [rows, cols], row stride ldx elements; rows may begin anywhere.
+ *   q:     device [rows, cols_pad / 2] bytes, the earlier of two values in the low half,
+ *          cols_pad = ceil(cols/256)*256, row stride ldq bytes (a multiple of 16); 16-byte
+ *          aligned; columns past cols are zeros.
+ *   scale: device bytes [ceil(cols_pad/512)][ceil(rows/16)][64][4], 4-byte aligned: row r's
+ *          and block b's e + 127 (255: NaN) at [b/16][r/16][16*(b%4) + r%16][b/4%4], the order
+ *          in which the projections read them. All of it is written, of rows and blocks that
+ *          do not exist as 0.
+ * rows may be 0; cols at most 33,553,920. No workspace; can be captured into a graph. */
+int h3hip_quant_rows_mx4(const void* x, int64_t ldx, int32_t rows, int32_t cols, void* q,
+                         int64_t ldq, void* scale, void* stream);
+
+/* The values that such rows stand for, as bf16, exactly (past bf16's range infinities):
+ * operands as h3hip_quant_rows_mx4 writes them, here with any ldq that is a multiple of 4 and
+ * q 4-byte aligned. x: device bf16 [rows, cols], row stride ldx elements; rows may begin
+ * anywhere, and nothing else is written. */
+int h3hip_dequant_rows_mx4(const void* q, int64_t ldq, const void* scale, int32_t rows,
+                           int32_t cols, void* x, int64_t ldx, void* stream);
+
+/* A projection on such operands, y = x . w^T: products of values exact, sums in fp32, one
+ * rounding to bf16. The 4-bit form of h3hip_out_proj, for any number of rows (0 and 1 too) and
+ * any width up to 16,776,960 of either and 2^23 tiles of 256 x 256 (H3HIP_EINVAL past them). A
+ * row's result does not depend on the other rows of the call.
+ *   x: device [rows, in_features/2] bytes, row stride ldx; w: device [out_features,
+ *      in_features/2], row stride ldw: as h3hip_quant_rows_mx4 writes them (16-byte aligned,
+ *      strides multiples of 16; scales of exactly these rows, from the first row on).
+ *   y: device bf16 [rows, out_features], row stride ldy elements; rows may begin
+ *      anywhere, and nothing else is written.
+ * Operands may pass 4 GiB; 256 rows of x or w must stay below 2 GiB.
+ * Declines unless in_features is a multiple of 256 (h3hip_quant_rows_mx4 pads with
+ * zeros). No workspace; can be captured into a graph. */
+int h3hip_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const void* w, int64_t ldw,
+                   const void* w_scale, int32_t in_features, int32_t out_features, int32_t rows,
+                   void* y, int64_t ldy, void* stream);
+
+/* h3hip_qkv_proj on such operands: the product of h3hip_proj_mx4 for Q | K | V rows of w,
+ * with the head norm and the rotation in its epilogue, in the rounding modes of
+ * h3hip_qkv_proj_i8: Q and K are h3hip_qk_norm_rope of h3hip_proj_mx4's result, bit for bit, or
+ * with H3HIP_ROUND_ONCE the norm and the rotation of the fp32 sums, rounded to bf16 only when
+ * they are stored; V is h3hip_proj_mx4's result, head-major.
+ *   x, x_scale, w, w_scale: as for h3hip_proj_mx4, w [3*heads*head_dim, hidden].
+ *   Everything else as for h3hip_qkv_proj (both gammas NULL: the plain product, head-major).
+ * Declines unless head_dim == 128, rot is 96 or 128 and hidden is a multiple of 256; any head
+ * count. seq_len and 3*heads*128 are limited as rows and width are for h3hip_proj_mx4. */
+int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const void* w, int64_t ldw,
+                       const void* w_scale, int32_t hidden, const void* q_gamma,
+                       const void* k_gamma, float eps, const void* rope_table, int32_t rot,
+                       int32_t rounding, int32_t seq_len, int32_t seq_pad, int32_t heads,
+                       int32_t head_dim, void* q_out, void* k_out, void* v_out, void* stream);
 
 /* -------------------------------------------------------------- attention */
 

@@ -57,7 +57,8 @@ SGPRS = list(range(64, 77))
 
 class Gen:
     """One tile shape's loop. The int8 loops (gen_gemm_i8_loop.py) are the same stream
-    with another product: a row's 128 bytes a step are then 128 values."""
+    with another product: a row's 128 bytes a step are then 128 values. The 4-bit loops
+    (gen_gemm_mx4_loop.py) have 256 values in them, and the values' scales beside them."""
     VARIANTS = VARIANTS
     MFMA = "v_mfma_f32_16x16x32_bf16"
     LABEL = "L_gemm"
@@ -121,6 +122,31 @@ class Gen:
     def w_calls(self, t, step):
         return [lambda i=i: self.load("w", t, i, step) for i in range(self.w_loads)]
 
+    # ---- what a product with more operands adds
+    def begin(self):
+        """After the resources are set up."""
+
+    def lead(self):
+        """Steps before the first whose loads are issued before the loop."""
+        return max(self.rw, self.rx)
+
+    def more_calls(self, t, step):
+        """Loads of step t's first sub-step beside those of W; t may lie before 0."""
+        return []
+
+    def needed(self, step):
+        """Tags of what has to have landed before the operands of a step are read."""
+        return ("w", step), ("x", step)
+
+    def product(self, t, u, na, mb):
+        c = self.C(na, mb)
+        return f"{self.MFMA} {c}, {self.A(u, na)}, {self.B(u, mb)}, {c}"
+
+    def inputs(self):
+        """(macro parameter, first register, how many)"""
+        return [("RA", self.ra, 2 * self.bases), ("RB", self.rb, 2 * self.bases),
+                ("XV", self.xv, self.x_loads), ("WV", self.wv, self.w_loads)]
+
     def wait_for(self, *tags):
         """vmcnt that leaves only what was issued after the last of tags."""
         last = max(i for i, t in enumerate(self.issued) if t in tags)
@@ -140,8 +166,8 @@ class Gen:
         return out
 
     # ---- one step
-    def sub_step(self, u, reads, calls):
-        """The MFMAs of sub-step u with the next sub-step's operand reads and
+    def sub_step(self, t, u, reads, calls):
+        """The MFMAs of sub-step u of step t with the next sub-step's operand reads and
         the loads spread between them."""
         n = self.na * self.mb
         reads, calls = list(reads), list(calls)
@@ -151,8 +177,7 @@ class Gen:
             self.emit("s_waitcnt lgkmcnt(0)")
         for k in range(n):
             na, mb = divmod(k, self.mb)
-            c = self.C(na, mb)
-            self.emit(f"{self.MFMA} {c}, {self.A(u, na)}, {self.B(u, mb)}, {c}")
+            self.emit(self.product(t, u, na, mb))
             # the reads over the first three quarters, so that they are back
             want = min(nr, -(-(k + 1) * nr * 4 // (3 * n)))
             while done_r < want:
@@ -174,11 +199,12 @@ class Gen:
 
     def step(self, t, vt, end):
         """Step t (unrolled) traced as step vt, with the exit test at its end."""
-        self.sub_step(0, self.reads(t, 1), self.w_calls(t - 1 + self.rw, vt - 1 + self.rw))
-        wait = self.wait_for(("w", vt + 1), ("x", vt + 1))
+        self.sub_step(t, 0, self.reads(t, 1),
+                      self.w_calls(t - 1 + self.rw, vt - 1 + self.rw) + self.more_calls(t, vt))
+        wait = self.wait_for(*self.needed(vt + 1))
         self.emit(f"s_waitcnt vmcnt({wait}) lgkmcnt(0)", "s_barrier")
         self.advance()
-        self.sub_step(1, self.reads(t + 1, 0), self.x_calls(t + self.rx, vt + self.rx))
+        self.sub_step(t, 1, self.reads(t + 1, 0), self.x_calls(t + self.rx, vt + self.rx))
         self.emit(f"s_add_u32 {SJ}, {SJ}, 1", f"s_cmp_eq_u32 {SJ}, %[steps]",
                   f"s_cbranch_scc1 {end}")
         return wait
@@ -193,6 +219,7 @@ class Gen:
         for i, r in enumerate(("w_lo", "w_hi", "w_rec")):
             em(f"s_mov_b32 s{68 + i}, %[{r}]")
         em("s_mov_b32 s71, 0x20000", f"s_mov_b32 {SJ}, 0")
+        self.begin()
 
         def first(which, step):
             off, rec = (SXO, "s66") if which == "x" else (SWO, "s70")
@@ -204,7 +231,9 @@ class Gen:
         # The loads before the loop, in the loop's order (x of step t + RX,
         # then W of step t + RW, for t before 0); the loop starts with W of
         # step RW - 1.
-        for t in range(-max(self.rw, self.rx), 0):
+        for t in range(-self.lead(), 0):
+            for c in self.more_calls(t, t):
+                em(*c())
             if t + self.rx >= 0:
                 first("x", t + self.rx)
             if t + self.rw >= 0 and t < -1:
@@ -214,7 +243,7 @@ class Gen:
            "s_cselect_b32 s70, s70, 0")
         for r in range(4 * self.na * self.mb):
             em(f"v_accvgpr_write_b32 a{r}, 0")
-        em(f"s_waitcnt vmcnt({self.wait_for(('w', 0), ('x', 0))})", "s_barrier")
+        em(f"s_waitcnt vmcnt({self.wait_for(*self.needed(0))})", "s_barrier")
         em(*self.reads(0, 0))
         em(f"{loop}:")
         waits = [self.step(t, t, end) for t in range(self.unroll)]
@@ -240,17 +269,15 @@ def render(gen=Gen, script="gen_gemm_loop.py", macro="H3_GEMM"):
         g = gen(name)
         lines = g.generate()
         body = " \\\n".join('  "' + ln + '\\n"' for ln in lines)
-        ins = [f'"{{v{at + i}}}"({arg}[{i}])'
-               for arg, at, n in (("RA", g.ra, 2 * g.bases), ("RB", g.rb, 2 * g.bases),
-                                  ("XV", g.xv, g.x_loads), ("WV", g.wv, g.w_loads))
-               for i in range(n)]
+        ins = [f'"{{v{at + i}}}"({arg}[{i}])' for arg, at, n in g.inputs() for i in range(n)]
+        args = ", ".join(arg for arg, _, _ in g.inputs())
         acc = [f'"=&{{a[{32 * i}:{32 * i + 31}]}}"(C[{i}])' for i in range(-(-na * mb // 8))]
         out += [f"// {32 * na} channels x {32 * mb} tokens: {len(lines)} lines.",
                 f"#define {macro}_LDS_{name} {g.lds}",
                 f"#define {macro}_BASES_{name} {g.bases}",
                 f"#define {macro}_LOOP_{name} \\\n" + body + "\n",
                 f"#define {macro}_OUT_{name}(C) " + ", ".join(acc),
-                f"#define {macro}_IN_{name}(RA, RB, XV, WV) " + ", ".join(ins),
+                f"#define {macro}_IN_{name}({args}) " + ", ".join(ins),
                 f"#define {macro}_CLOBBERS_{name} " + ", ".join(f'"{r}"' for r in g.clobbers())]
     return "\n".join(out) + "\n"
 

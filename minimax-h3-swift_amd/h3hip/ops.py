@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -441,6 +442,203 @@ def _check_norm_rope(device, S, head_dim, q_gamma, k_gamma, table, rounding) -> 
         raise ValueError(f"table must be a contiguous {dt} [>= {S}, rot/2, 2, 2] tensor on {device} "
                          "(rope_table() with the same rounding mode)")
     return 2 * table.shape[1]
+
+
+# ------------------------------------------- microscaled 4-bit projections
+
+_U8 = torch.uint8
+MX4_BLOCK = 32                   # consecutive values of a row that share a scale
+
+
+class Mx4Rows(NamedTuple):
+    """Rows of microscaled 4-bit floats (MXFP4): what the 4-bit projections multiply.
+
+    values: [S, cols padded to a multiple of 256, / 2] uint8, two values a byte, the earlier in
+    the low half (row stride free). scale: [slabs, ceil(S/16), 64, 4] uint8, the blocks' biased
+    exponents in the order in which the kernels read them: row r's and block b's at
+    [b // 16, r // 16, 16 * (b % 4) + r % 16, b // 4 % 4]. cols: values of a row.
+    quant_rows_mx4() makes them of bf16 rows, pack() of what a checkpoint holds."""
+    values: torch.Tensor
+    scale: torch.Tensor
+    cols: int
+
+    @property
+    def shape(self):
+        return self.values.shape[0], self.cols
+
+    @classmethod
+    def pack(cls, codes: torch.Tensor, exponents: torch.Tensor, cols: int | None = None):
+        """Of row-major MXFP4 (codes [S, n/2] uint8, exponents [S, ceil(n/32)] uint8), laid out
+        once; values past ``cols`` (n by default) become zeros."""
+        if codes.dim() != 2 or codes.dtype != _U8 or codes.shape[1] == 0:
+            raise ValueError(f"codes must be uint8 [S, n/2], got {codes.dtype} {tuple(codes.shape)}")
+        S, n = codes.shape[0], 2 * codes.shape[1]
+        blocks = (n + MX4_BLOCK - 1) // MX4_BLOCK
+        if exponents.dtype != _U8 or tuple(exponents.shape) != (S, blocks):
+            raise ValueError(f"exponents must be uint8 [{S}, {blocks}], got {exponents.dtype} "
+                             f"{tuple(exponents.shape)}")
+        _require_same_device(codes.device, exponents=exponents)
+        cols = n if cols is None else cols
+        if not 0 < cols <= n:
+            raise ValueError(f"cols must be in 1..{n}, got {cols}")
+        values = codes.new_zeros((S, (cols + 255) // 256 * 128))
+        used = (cols + 1) // 2
+        values[:, :used] = codes[:, :used]
+        if cols % 2:
+            values[:, used - 1] &= 15
+        blocks, slabs, groups = (cols + MX4_BLOCK - 1) // MX4_BLOCK, (cols + 511) // 512, (S + 15) // 16
+        rows = codes.new_zeros((16 * groups, 16 * slabs))
+        rows[:S, :blocks] = exponents[:, :blocks]
+        # [group, row, slab, byte, quarter] -> [slab, group, quarter, row, byte]
+        scale = rows.view(groups, 16, slabs, 4, 4).permute(2, 0, 4, 1, 3)
+        return cls(values, scale.reshape(slabs, groups, 64, 4).contiguous(), cols)
+
+    def exponents(self) -> torch.Tensor:
+        """The biased exponents row-major, [S, ceil(cols/32)] uint8: what pack() takes."""
+        slabs, groups = self.scale.shape[:2]
+        rows = self.scale.view(slabs, groups, 4, 16, 4).permute(1, 3, 0, 4, 2)
+        rows = rows.reshape(16 * groups, 16 * slabs)
+        return rows[:self.values.shape[0], :(self.cols + MX4_BLOCK - 1) // MX4_BLOCK].contiguous()
+
+
+def _mx4_sizes(S: int, K: int):
+    """(bytes of a row of values, shape of the scales)."""
+    return (K + 255) // 256 * 128, ((K + 511) // 512, (S + 15) // 16, 64, 4)
+
+
+def _mx4_operand(name: str, t, device: torch.device | None = None):
+    """Checks an Mx4Rows; returns (device, rows, bytes of a row, row stride in bytes)."""
+    if not isinstance(t, Mx4Rows):
+        raise ValueError(f"{name} must be an Mx4Rows (quant_rows_mx4() or Mx4Rows.pack()), "
+                         f"got {type(t).__name__}")
+    v, s, cols = t
+    ld = _rows(f"{name}.values", v, _U8)
+    S, n = v.shape
+    if S > _INT32_MAX or not 0 < cols <= _INT32_MAX:
+        raise ValueError(f"{name} must have sizes from 1 to below 2^31, got {S} x {cols}")
+    width, shape = _mx4_sizes(S, cols)
+    if n != width:
+        raise ValueError(f"{name}.values must be [{S}, {width}] for {cols} columns, got "
+                         f"{tuple(v.shape)}")
+    if s.dtype is not _U8 or s.shape != shape or not s.is_contiguous():
+        raise ValueError(f"{name}.scale must be contiguous uint8 {shape}, got {s.dtype} "
+                         f"{tuple(s.shape)}")
+    if not v.is_cuda:
+        raise ValueError(f"{name} must be on a GPU (no host fallback exists)")
+    device = v.device if device is None else device
+    if v.device != device or s.device != device:
+        raise ValueError(f"{name} must be on {device}, got {v.device} and {s.device}")
+    return device, S, n, ld
+
+
+def quant_rows_mx4(x: torch.Tensor, out: Mx4Rows | None = None) -> Mx4Rows:
+    """Rows of bf16 rounded to 4-bit floats, a power of two for every 32 consecutive values.
+
+    x: [S, K] bf16 (row stride free, unit column stride): the activations of a 4-bit
+    projection, or its weights, rounded once. A block holding an infinity or a NaN gets the
+    scale NaN. ``out`` is an Mx4Rows of these sizes to write into."""
+    ldx = _rows("x", x, _BF16)
+    S, K = x.shape
+    if K == 0:
+        raise ValueError("x must be [S, K > 0]")
+    if S > _INT32_MAX or K > _INT32_MAX:
+        _require_int32("x", x)
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor (no host fallback exists)")
+    device = x.device
+    if out is None:
+        width, ldq = (K + 255) // 256 * 128, (K + 255) // 256 * 128
+        out = Mx4Rows(_empty(S, width, dtype=_U8, device=device),
+                      _empty((K + 511) // 512, (S + 15) // 16, 64, 4, dtype=_U8, device=device), K)
+    else:
+        _, rows, _, ldq = _mx4_operand("out", out, device)
+        if (rows, out.cols) != (S, K):
+            raise ValueError(f"out must hold [{S}, {K}], got {out.shape}")
+    _run(L.lib().h3hip_quant_rows_mx4, device, x.data_ptr(), ldx, S, K, out.values.data_ptr(), ldq,
+         out.scale.data_ptr())
+    return out
+
+
+def dequant_rows_mx4(rows: Mx4Rows, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values that 4-bit rows stand for, [S, cols] bf16, exactly."""
+    device, S, _, ldq = _mx4_operand("rows", rows)
+    if out is None:
+        out = _empty(S, rows.cols, dtype=_BF16, device=device)
+    elif out.shape != (S, rows.cols):
+        raise ValueError(f"out must be [{S}, {rows.cols}], got {tuple(out.shape)}")
+    ldx = _rows("out", out, _BF16)
+    _require_same_device(device, out=out)
+    _run(L.lib().h3hip_dequant_rows_mx4, device, rows.values.data_ptr(), ldq, rows.scale.data_ptr(),
+         S, rows.cols, out.data_ptr(), ldx)
+    return out
+
+
+def _mx4_product(x, w):
+    """Checks the operands of a 4-bit product, rounding a bf16 x; returns (x, device, S, bytes of
+    a row, N, ldx, ldw)."""
+    device, N, n, ldw = _mx4_operand("w", w)
+    if isinstance(x, torch.Tensor):
+        if x.dim() != 2 or x.shape[1] != w.cols:
+            raise ValueError(f"x must be [S, {w.cols}], got {tuple(x.shape)}")
+        _require_same_device(device, x=x)
+        x = quant_rows_mx4(x)
+        return x, device, x.values.shape[0], n, N, n, ldw
+    _, S, nx, ldx = _mx4_operand("x", x, device)
+    if x.cols != w.cols:
+        raise ValueError(f"w must hold [out, {x.cols}], got {w.shape}")
+    return x, device, S, n, N, ldx, ldw
+
+
+def proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, out: torch.Tensor | None = None):
+    """A projection on 4-bit operands: y = x . w^T with fp32 sums.
+
+    x: [S, K] bf16, rounded by quant_rows_mx4() on the way, or an Mx4Rows; w: [N, K], rounded
+    or laid out once (S and N up to 16,776,960). Returns y [S, N] bf16 (or writes ``out``, any
+    row stride), or None when declined."""
+    x, device, S, n, N, ldx, ldw = _mx4_product(x, w)
+    if out is None:
+        out = _empty(S, N, dtype=_BF16, device=device)
+        ldy = N
+    else:
+        ldy = _rows("out", out, _BF16)
+        if out.shape != (S, N):
+            raise ValueError(f"out must be [{S}, {N}], got {tuple(out.shape)}")
+        _require_same_device(device, out=out)
+    rc = _run(L.lib().h3hip_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
+              w.values.data_ptr(), ldw, w.scale.data_ptr(), 2 * n, N, S, out.data_ptr(), ldy)
+    return None if rc == L.DECLINED else out
+
+
+def qkv_proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, q_gamma: torch.Tensor | None = None,
+                 k_gamma: torch.Tensor | None = None, table: torch.Tensor | None = None, *,
+                 heads: int, head_dim: int = 128, eps: float = 1e-6, seq_pad: int | None = None,
+                 rounding: int = L.ROUND_REFERENCE, out=None):
+    """qkv_proj() on 4-bit operands (x and w as for proj_mx4(), w [3*heads*head_dim, hidden]):
+    the QKV product with the Q/K norm + RoPE in its epilogue. ROUND_REFERENCE and ROUND_FP32
+    normalise the bf16 product, as qkv_proj() does; ROUND_ONCE keeps it in fp32 up to the one
+    rounding of Q and K. Returns (q, k, v) as [heads, seq_pad, head_dim] bf16, or None when the
+    geometry is declined."""
+    x, device, S, n, N, ldx, ldw = _mx4_product(x, w)
+    if N != 3 * heads * head_dim:
+        raise ValueError(f"w must hold [{3 * heads * head_dim}, {w.cols}], got {w.shape}")
+    seq_pad = seq_pad or (S + L.TILE - 1) // L.TILE * L.TILE
+    if q_gamma is None and k_gamma is None:
+        rot, gq, gk, tab = head_dim, None, None, None
+    else:
+        rot = _check_norm_rope(device, S, head_dim, q_gamma, k_gamma, table, rounding)
+        gq, gk, tab = q_gamma.data_ptr(), k_gamma.data_ptr(), table.data_ptr()
+    shape = (heads, seq_pad, head_dim)
+    if out is None:
+        out = _empty(3, heads, seq_pad, head_dim, dtype=_BF16, device=device).unbind(0)
+    else:
+        out = tuple(out)
+        for t in out:
+            _require_out(t, shape, device)
+    q_out, k_out, v_out = out
+    rc = _run(L.lib().h3hip_qkv_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
+              w.values.data_ptr(), ldw, w.scale.data_ptr(), 2 * n, gq, gk, eps, tab, rot, rounding,
+              S, seq_pad, heads, head_dim, q_out.data_ptr(), k_out.data_ptr(), v_out.data_ptr())
+    return None if rc == L.DECLINED else out
 
 
 # -------------------------------------------------------------------- attention
