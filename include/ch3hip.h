@@ -394,6 +394,50 @@ int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const vo
                        int32_t rounding, int32_t seq_len, int32_t seq_pad, int32_t heads,
                        int32_t head_dim, void* q_out, void* k_out, void* v_out, void* stream);
 
+/* ---------------------------------- norm, modulation, gate and residual */
+
+/* A norm over the hidden width with its modulation: of a row x of segment s
+ *   x rsqrt(mean x^2 + eps) gamma (1 + scale[s]) + shift[s]
+ * All tables device bf16 and optional: gamma [hidden] (NULL: 1), scale and shift
+ * [segments, hidden] with row strides in elements (NULL: 0). */
+typedef struct {
+  const void* gamma;
+  const void* scale;
+  const void* shift;
+  int64_t ld_scale;
+  int64_t ld_shift;
+} h3hip_norm;
+
+/* The norm before a block's attention, of the residual stream: H3RMSNorm
+ * (Sources/H3Modules/Modulation.swift:116-120) over the hidden width, modulated. fp32 up to
+ * the one rounding of h.
+ *   x: device bf16 [rows, hidden], row stride ldx; h: device bf16 [rows, hidden], row stride
+ *      ldh; rows may begin anywhere. h may be x (the same address and stride), and no other
+ *      overlap is allowed.
+ *   starts: host, the first row of each segment, not descending, starts[0] = 0; NULL: one
+ *      segment. Segments of no rows, and starts past the last row, are fine. Travels by value.
+ *   segments: 1 to 16.
+ * rows may be 0. A row whose squares pass fp32 (magnitudes of 1e18 and more) comes out as its
+ * shift. No workspace; can be captured into a graph. Declines hidden above 16,384. */
+int h3hip_norm_modulate(const void* x, int64_t ldx, int32_t rows, int32_t hidden,
+                        const h3hip_norm* norm, float eps, const int32_t* starts,
+                        int32_t segments, void* h, int64_t ldh, void* stream);
+
+/* The end of a block's half: of the residual stream x and its output y
+ *   r = residual_scale x + gate[s] z, z = y or, with post_gamma, y rsqrt(mean y^2 + eps) post_gamma
+ * and, with next, the norm of r that the next half begins with, h (of the fp32 r, which is
+ * rounded to bf16 only as r). fp32 up to those roundings.
+ *   x, y, r, h: device bf16 [rows, hidden], row strides in elements; rows may begin anywhere.
+ *      r or h may be x or y (the same address and stride), and no other overlap is allowed.
+ *   gate: device bf16 [segments, hidden], row stride ld_gate (NULL: 1); post_gamma: device
+ *      bf16 [hidden] or NULL. next: a host struct or NULL (h unused).
+ * Everything else as for h3hip_norm_modulate. */
+int h3hip_gated_residual(const void* x, int64_t ldx, const void* y, int64_t ldy, int32_t rows,
+                         int32_t hidden, const void* gate, int64_t ld_gate,
+                         const void* post_gamma, float residual_scale, const h3hip_norm* next,
+                         float eps, const int32_t* starts, int32_t segments, void* r, int64_t ldr,
+                         void* h, int64_t ldh, void* stream);
+
 /* -------------------------------------------------------------- attention */
 
 /* Block-sparse attention over the plan's active tiles: for each query row,

@@ -77,6 +77,17 @@ class ViewC(ctypes.Structure):
     ]
 
 
+class NormC(ctypes.Structure):
+    """h3hip_norm: device tables of a modulated norm."""
+    _fields_ = [
+        ("gamma", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("shift", ctypes.c_void_p),
+        ("ld_scale", ctypes.c_int64),
+        ("ld_shift", ctypes.c_int64),
+    ]
+
+
 # Every symbol include/ch3hip.h declares, with (restype, argtypes).
 SIGNATURES = {
     "h3hip_device_supported": (ctypes.c_int, [ctypes.c_int32]),
@@ -133,6 +144,14 @@ SIGNATURES = {
                                           ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                           ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _vp,
                                           _vp, _vp, _vp]),
+    "h3hip_norm_modulate": (ctypes.c_int, [_vp, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                           ctypes.POINTER(NormC), ctypes.c_float, _i32p,
+                                           ctypes.c_int32, _vp, ctypes.c_int64, _vp]),
+    "h3hip_gated_residual": (ctypes.c_int, [_vp, ctypes.c_int64, _vp, ctypes.c_int64,
+                                            ctypes.c_int32, ctypes.c_int32, _vp, ctypes.c_int64,
+                                            _vp, ctypes.c_float, ctypes.POINTER(NormC),
+                                            ctypes.c_float, _i32p, ctypes.c_int32, _vp,
+                                            ctypes.c_int64, _vp, ctypes.c_int64, _vp]),
     "h3hip_bsattn_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int32, ctypes.c_int32,
                                         ctypes.c_float, _vp, ctypes.c_int32, _vp]),
     "h3hip_bsattn_fwd_strided": (ctypes.c_int, [_vp, ctypes.POINTER(ViewC),

@@ -641,6 +641,132 @@ def qkv_proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, q_gamma: torch.Tensor | 
     return None if rc == L.DECLINED else out
 
 
+# -------------------------------------- norm, modulation, gate and residual
+
+def _norm_rows(name: str, t: torch.Tensor, shape, device) -> int:
+    """Checks bf16 rows of a norm; returns their stride."""
+    ld = _rows(name, t, _BF16)
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    return ld
+
+
+def _norm_gamma(name: str, t, hidden: int, device):
+    if t is None:
+        return None
+    if t.dtype is not _BF16 or t.shape != (hidden,) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be contiguous bfloat16 [{hidden}] on {device}")
+    return t.data_ptr()
+
+
+def _norm_table(name: str, t, segments: int, hidden: int, device):
+    """(address, row stride) of a modulation [segments, hidden] or, of one segment, [hidden]."""
+    if t is None:
+        return None, hidden
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    if (t.dtype is not _BF16 or t.shape != (segments, hidden) or t.device != device
+            or (t.stride(1) != 1 and hidden > 1)):
+        raise ValueError(f"{name} must be bfloat16 [{segments}, {hidden}] on {device} with unit "
+                         f"column stride, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr(), (t.stride(0) if segments > 1 else hidden)
+
+
+def _norm_c(gamma, scale, shift, segments, hidden, device) -> L.NormC:
+    scale, ld_scale = _norm_table("scale", scale, segments, hidden, device)
+    shift, ld_shift = _norm_table("shift", shift, segments, hidden, device)
+    return L.NormC(_norm_gamma("gamma", gamma, hidden, device), scale, shift, ld_scale, ld_shift)
+
+
+def _segments(starts):
+    """(host array or None, how many) of the segments' first rows."""
+    if starts is None:
+        return None, 1
+    n = len(starts)
+    if not 1 <= n <= 16:
+        raise ValueError(f"segments must be 1 to 16 first rows, got {n}")
+    if any(not 0 <= int(v) <= _INT32_MAX for v in starts):
+        raise ValueError(f"segments must be rows from 0 to below 2^31, got {list(starts)}")
+    return (ctypes.c_int32 * n)(*map(int, starts)), n
+
+
+def _norm_input(x: torch.Tensor):
+    ld = _rows("x", x, _BF16)
+    S, hidden = x.shape
+    if hidden == 0:
+        raise ValueError("x must be [S, hidden > 0]")
+    if S > _INT32_MAX or hidden > _INT32_MAX:
+        _require_int32("x", x)
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor (no host fallback exists)")
+    return ld, S, hidden, x.device
+
+
+def norm_modulate(x: torch.Tensor, gamma: torch.Tensor | None = None,
+                  scale: torch.Tensor | None = None, shift: torch.Tensor | None = None, *,
+                  segments=None, eps: float = 1e-6, out: torch.Tensor | None = None):
+    """The norm before a block: x rsqrt(mean x^2 + eps) gamma (1 + scale[s]) + shift[s].
+
+    x: [S, hidden] bf16 (row stride free). gamma: [hidden]; scale, shift: [segments, hidden] bf16
+    (or [hidden], of one segment), each optional. segments: the first row of each, not
+    descending, from 0 on (None: one segment). Returns h [S, hidden] bf16 (or writes ``out``, any
+    row stride; x itself is allowed), or None when declined (hidden above 16,384)."""
+    ldx, S, hidden, device = _norm_input(x)
+    starts, n = _segments(segments)
+    norm = _norm_c(gamma, scale, shift, n, hidden, device)
+    if out is None:
+        out, ldh = _empty(S, hidden, dtype=_BF16, device=device), hidden
+    else:
+        ldh = _norm_rows("out", out, (S, hidden), device)
+    rc = _run(L.lib().h3hip_norm_modulate, device, x.data_ptr(), ldx, S, hidden, norm, eps, starts,
+              n, out.data_ptr(), ldh)
+    return None if rc == L.DECLINED else out
+
+
+def gated_residual(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None = None, *,
+                   post_gamma: torch.Tensor | None = None, residual_scale: float = 1.0,
+                   segments=None, eps: float = 1e-6, next_norm: dict | None = None, out=None):
+    """The end of a block's half: r = residual_scale x + gate[s] z, z being y or, with
+    post_gamma, y rsqrt(mean y^2 + eps) post_gamma.
+
+    x, y: [S, hidden] bf16 (row strides free); gate: [segments, hidden] bf16 (or [hidden], of one
+    segment) or None (1); segments as for norm_modulate(). next_norm: a dict of the gamma,
+    scale and shift (any of them) of the norm that the next half begins with; it is taken of r
+    before r is rounded. Returns r, with next_norm (r, h), [S, hidden] bf16 each, or None when
+    declined (hidden above 16,384). ``out`` is r, or (r, h), to write into: any row stride, x or
+    y themselves are allowed."""
+    ldx, S, hidden, device = _norm_input(x)
+    ldy = _norm_rows("y", y, (S, hidden), device)
+    starts, n = _segments(segments)
+    gate, ld_gate = _norm_table("gate", gate, n, hidden, device)
+    post = _norm_gamma("post_gamma", post_gamma, hidden, device)
+    norm = h = None
+    ldh = hidden
+    if next_norm is not None:
+        wrong = set(next_norm) - {"gamma", "scale", "shift"}
+        if wrong:
+            raise ValueError(f"next_norm takes gamma, scale and shift, got {sorted(wrong)}")
+        norm = _norm_c(next_norm.get("gamma"), next_norm.get("scale"), next_norm.get("shift"), n,
+                       hidden, device)
+    if out is None:
+        r, ldr = _empty(S, hidden, dtype=_BF16, device=device), hidden
+        if norm is not None:
+            h = _empty(S, hidden, dtype=_BF16, device=device)
+    else:
+        r, h = out if norm is not None else (out, None)
+        ldr = _norm_rows("out", r, (S, hidden), device)
+        if h is not None:
+            ldh = _norm_rows("out[1]", h, (S, hidden), device)
+    rc = _run(L.lib().h3hip_gated_residual, device, x.data_ptr(), ldx, y.data_ptr(), ldy, S, hidden,
+              gate, ld_gate, post, residual_scale, norm, eps, starts, n, r.data_ptr(), ldr,
+              None if h is None else h.data_ptr(), ldh)
+    if rc == L.DECLINED:
+        return None
+    return r if norm is None else (r, h)
+
+
 # -------------------------------------------------------------------- attention
 
 def _head_major_qkv(plan: TilePlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
