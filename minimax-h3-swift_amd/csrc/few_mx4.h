@@ -1,0 +1,21 @@
+// Arguments of the 4-bit projection of one or two bf16 rows (few_mx4.hip) and its launch.
+#pragma once
+
+#include "common.h"
+
+namespace h3hip {
+
+struct FewMx4Args {
+  const uint16_t* __restrict__ x;        // [rows, cols], row stride ldx elements
+  const uint8_t* __restrict__ w;         // [n_total, units * 128], row stride ldw bytes
+  const uint8_t* __restrict__ w_scale;
+  uint16_t* __restrict__ y;              // [rows, n_total], row stride ldy elements
+  int64_t ldx, ldw, ldy;
+  int32_t rows, cols, units, n_total;    // units: of 256 values of the reduction
+};
+
+// Whether few_mx4_kernel takes a call of these sizes.
+bool few_mx4_takes(int32_t rows, int32_t cols);
+int launch_few_mx4(const FewMx4Args& a, hipStream_t stream);
+
+}  // namespace h3hip

@@ -18,7 +18,7 @@
 #include <algorithm>
 #include <climits>
 
-#include "common.h"
+#include "mx4_block.h"
 
 namespace h3hip {
 
@@ -26,11 +26,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnitRows = 16, kUnitCols = 512;
-constexpr uint32_t kAbs2 = 0x7fff7fffu;
-constexpr uint32_t kNanScale = 255u;
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct QuantMx4Args {
   const uint16_t* __restrict__ x;
@@ -39,31 +34,6 @@ struct QuantMx4Args {
   int64_t ldx, ldq;
   int32_t rows, cols, cols_pad, row0;   // row0: the launch's first row, a multiple of 16
 };
-
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
-                                                                __builtin_bit_cast(u16x2, b)));
-}
-
-// 8 elements from column k on, zeros past cols. Rows may begin anywhere.
-__device__ __forceinline__ u32x4 load8(const uint16_t* row, int64_t k, int cols) {
-  if (k + 8 <= cols) return *reinterpret_cast<const u32x4_any*>(row + k);
-  u32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const uint32_t lo = k + 2 * i < cols ? row[k + 2 * i] : 0u;
-    const uint32_t hi = k + 2 * i + 1 < cols ? row[k + 2 * i + 1] : 0u;
-    v[i] = lo | hi << 16;
-  }
-  return v;
-}
-
-__device__ __forceinline__ bf16x2 pair(uint32_t w) { return __builtin_bit_cast(bf16x2, w); }
-
-// The fp32 2^(byte - 127); 0 is 2^-127, a subnormal.
-__device__ __forceinline__ float scale_of(uint32_t byte) {
-  return __uint_as_float(byte == 0 ? 1u << 22 : byte << 23);
-}
 
 __global__ __launch_bounds__(kThreads) void quant_mx4_kernel(QuantMx4Args a) {
   __shared__ uint32_t scales[64];
@@ -75,30 +45,13 @@ __global__ __launch_bounds__(kThreads) void quant_mx4_kernel(QuantMx4Args a) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {              // rows wave, wave + 4, ...
     const int64_t r = r0 + wave + 4 * i;
-    v[i] = r < a.rows ? load8(a.x + r * a.ldx, k, a.cols) : u32x4{0u, 0u, 0u, 0u};
+    v[i] = r < a.rows ? load_bf16x8(a.x + r * a.ldx, k, a.cols) : u32x4{0u, 0u, 0u, 0u};
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const int row = wave + 4 * i;
-    // Magnitudes of bf16 compare as whole numbers; infinities and NaN lie above the rest.
-    uint32_t m2 = 0;
-#pragma unroll
-    for (int h = 0; h < 4; h++) m2 = max_u16x2(m2, v[i][h] & kAbs2);
-    uint32_t top = max(m2 & 0xffffu, m2 >> 16);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-    // A block that holds an infinity or a NaN has no such form: its scale is NaN, so that
-    // whatever is multiplied with it shows, and its values are zeros.
-    const bool finite = top < 0x7f80u;
-    const uint32_t e = top >> 7;             // biased exponent; 0: subnormals and zero
-    const uint32_t byte = finite ? (e > 2 ? e - 2 : 0u) : kNanScale;
-    const float s = scale_of(finite ? byte : 127u);
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, pair(v[i][0]), s, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, pair(v[i][1]), s, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, pair(v[i][2]), s, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, pair(v[i][3]), s, 3);
-    if (!finite) codes = 0;
+    uint32_t byte;
+    const uint32_t codes = mx4_codes(v[i], byte);
     if (r0 + row < a.rows && k < a.cols_pad)
       *reinterpret_cast<uint32_t*>(a.q + (r0 + row) * a.ldq + k / 2) = codes;
     if ((lane & 3) == 0)
@@ -140,13 +93,13 @@ __global__ __launch_bounds__(kThreads) void dequant_mx4_kernel(DequantMx4Args a)
   for (int i = 0; i < 4; i++) {
     const int64_t r = r0 + wave + 4 * i;
     if (r >= a.rows) continue;
-    const float s = scale_of(bytes[i]);
+    const float s = mx4_scale(bytes[i]);
     u32x4 v;
     v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[i], s, 0));
     v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[i], s, 1));
     v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[i], s, 2));
     v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[i], s, 3));
-    if (bytes[i] == kNanScale) v = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    if (bytes[i] == kMx4NanScale) v = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
     uint16_t* dst = a.x + r * a.ldx + k;
     if (k + 8 <= a.cols) {
       *reinterpret_cast<u32x4_any*>(dst) = v;

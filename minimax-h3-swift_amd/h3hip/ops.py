@@ -8,6 +8,7 @@ can run its own dense path, exactly as the reference's backends decline.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -501,6 +502,23 @@ class Mx4Rows(NamedTuple):
         return rows[:self.values.shape[0], :(self.cols + MX4_BLOCK - 1) // MX4_BLOCK].contiguous()
 
 
+def _bf16_rows(x: torch.Tensor):
+    """Checks the bf16 rows that a call begins with; returns (stride, rows, columns, device)."""
+    if x.dim() == 2 and x.dtype is _BF16 and x.is_cuda:
+        (S, K), (ld, step) = x.shape, x.stride()
+        if step == 1 and 0 < K <= _INT32_MAX and S <= _INT32_MAX:
+            return (ld if S > 1 else K), S, K, x.device
+    ld = _rows("x", x, _BF16)
+    S, K = x.shape
+    if K == 0:
+        raise ValueError("x must be [S, K > 0]")
+    if S > _INT32_MAX or K > _INT32_MAX:
+        _require_int32("x", x)
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor (no host fallback exists)")
+    return ld, S, K, x.device
+
+
 def _mx4_sizes(S: int, K: int):
     """(bytes of a row of values, shape of the scales)."""
     return (K + 255) // 256 * 128, ((K + 511) // 512, (S + 15) // 16, 64, 4)
@@ -512,6 +530,13 @@ def _mx4_operand(name: str, t, device: torch.device | None = None):
         raise ValueError(f"{name} must be an Mx4Rows (quant_rows_mx4() or Mx4Rows.pack()), "
                          f"got {type(t).__name__}")
     v, s, cols = t
+    if v.dim() == 2 and v.dtype is _U8 and s.dtype is _U8 and v.is_cuda and 0 < cols <= _INT32_MAX:
+        (S, n), (ld, step) = v.shape, v.stride()
+        where = v.device
+        if (S <= _INT32_MAX and n == (cols + 255) // 256 * 128 and step == 1
+                and (device is None or where == device) and s.device == where
+                and s.shape == ((cols + 511) // 512, (S + 15) // 16, 64, 4) and s.is_contiguous()):
+            return where, S, n, (ld if S > 1 else n)
     ld = _rows(f"{name}.values", v, _U8)
     S, n = v.shape
     if S > _INT32_MAX or not 0 < cols <= _INT32_MAX:
@@ -537,18 +562,10 @@ def quant_rows_mx4(x: torch.Tensor, out: Mx4Rows | None = None) -> Mx4Rows:
     x: [S, K] bf16 (row stride free, unit column stride): the activations of a 4-bit
     projection, or its weights, rounded once. A block holding an infinity or a NaN gets the
     scale NaN. ``out`` is an Mx4Rows of these sizes to write into."""
-    ldx = _rows("x", x, _BF16)
-    S, K = x.shape
-    if K == 0:
-        raise ValueError("x must be [S, K > 0]")
-    if S > _INT32_MAX or K > _INT32_MAX:
-        _require_int32("x", x)
-    if not x.is_cuda:
-        raise ValueError("x must be a GPU tensor (no host fallback exists)")
-    device = x.device
+    ldx, S, K, device = _bf16_rows(x)
     if out is None:
-        width, ldq = (K + 255) // 256 * 128, (K + 255) // 256 * 128
-        out = Mx4Rows(_empty(S, width, dtype=_U8, device=device),
+        ldq = (K + 255) // 256 * 128
+        out = Mx4Rows(_empty(S, ldq, dtype=_U8, device=device),
                       _empty((K + 511) // 512, (S + 15) // 16, 64, 4, dtype=_U8, device=device), K)
     else:
         _, rows, _, ldq = _mx4_operand("out", out, device)
@@ -573,29 +590,56 @@ def dequant_rows_mx4(rows: Mx4Rows, out: torch.Tensor | None = None) -> torch.Te
     return out
 
 
-def _mx4_product(x, w):
-    """Checks the operands of a 4-bit product, rounding a bf16 x; returns (x, device, S, bytes of
-    a row, N, ldx, ldw)."""
-    device, N, n, ldw = _mx4_operand("w", w)
-    if isinstance(x, torch.Tensor):
-        if x.dim() != 2 or x.shape[1] != w.cols:
+@functools.lru_cache(maxsize=1024)
+def _mx4_workspace(S: int, K: int, heads: int) -> int:
+    return L.lib().h3hip_linear_mx4_workspace(S, K, heads)
+
+
+def _mx4_operands(x, w):
+    """Checks the operands of a 4-bit product, x in bf16 or an Mx4Rows; returns
+    (device, S, N, x's row stride, w's)."""
+    bf16 = isinstance(x, torch.Tensor)
+    if type(w) is Mx4Rows and (bf16 or type(x) is Mx4Rows):
+        v, s, K = w
+        xv = x if bf16 else x.values
+        if v.dim() == xv.dim() == 2:
+            (S, k), (N, n) = xv.shape, v.shape
+            (ldx, step), (ldw, step_w) = xv.stride(), v.stride()
+            device = xv.device
+            # The common case in one test (2 us less of a call that can be as short as 10); what
+            # of it is refused, one by one, below.
+            if (0 < K <= _INT32_MAX and S <= _INT32_MAX and N <= _INT32_MAX
+                    and n == (K + 255) // 256 * 128 and v.dtype is _U8 and s.dtype is _U8
+                    and step == 1 and step_w == 1 and s.is_contiguous() and xv.is_cuda
+                    and v.device == device and s.device == device
+                    and s.shape == ((K + 511) // 512, (N + 15) // 16, 64, 4)
+                    and (k == K and xv.dtype is _BF16 if bf16 else
+                         k == n and x.cols == K and _mx4_operand("x", x, device))):
+                return device, S, N, (ldx if S > 1 else (k + 15) // 16 * 16), (ldw if N > 1 else n)
+    if bf16:
+        ldx = _rows("x", x, _BF16)
+        device, N, _, ldw = _mx4_operand("w", w)
+        if x.shape[1] != w.cols:
             raise ValueError(f"x must be [S, {w.cols}], got {tuple(x.shape)}")
+        if x.shape[0] > _INT32_MAX:
+            _require_int32("x", x)
         _require_same_device(device, x=x)
-        x = quant_rows_mx4(x)
-        return x, device, x.values.shape[0], n, N, n, ldw
-    _, S, nx, ldx = _mx4_operand("x", x, device)
+        return device, x.shape[0], N, ldx, ldw
+    device, S, _, ldx = _mx4_operand("x", x)
+    _, N, _, ldw = _mx4_operand("w", w, device)
     if x.cols != w.cols:
         raise ValueError(f"w must hold [out, {x.cols}], got {w.shape}")
-    return x, device, S, n, N, ldx, ldw
+    return device, S, N, ldx, ldw
 
 
 def proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, out: torch.Tensor | None = None):
     """A projection on 4-bit operands: y = x . w^T with fp32 sums.
 
-    x: [S, K] bf16, rounded by quant_rows_mx4() on the way, or an Mx4Rows; w: [N, K], rounded
-    or laid out once (S and N up to 16,776,960). Returns y [S, N] bf16 (or writes ``out``, any
-    row stride), or None when declined."""
-    x, device, S, n, N, ldx, ldw = _mx4_product(x, w)
+    x: [S, K] bf16 (row stride free), rounded as by quant_rows_mx4() on the way, or an
+    Mx4Rows; w: [N, K], rounded or laid out once (S and N up to 16,776,960). One or two bf16
+    rows take one launch, whose sums add in another order than those of more. Returns y [S, N]
+    bf16 (or writes ``out``, any row stride), or None when declined."""
+    device, S, N, ldx, ldw = _mx4_operands(x, w)
     if out is None:
         out = _empty(S, N, dtype=_BF16, device=device)
         ldy = N
@@ -604,8 +648,16 @@ def proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, out: torch.Tensor | None = N
         if out.shape != (S, N):
             raise ValueError(f"out must be [{S}, {N}], got {tuple(out.shape)}")
         _require_same_device(device, out=out)
-    rc = _run(L.lib().h3hip_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
-              w.values.data_ptr(), ldw, w.scale.data_ptr(), 2 * n, N, S, out.data_ptr(), ldy)
+    v, s, K = w
+    if type(x) is Mx4Rows:
+        rc = _run(L.lib().h3hip_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
+                  v.data_ptr(), ldw, s.data_ptr(), 2 * v.shape[1], N, S, out.data_ptr(), ldy)
+    else:
+        size, work = _mx4_workspace(S, K, 0), None
+        if size:
+            work = _empty(size, dtype=_U8, device=device)
+        rc = _run(L.lib().h3hip_linear_mx4, device, x.data_ptr(), ldx, v.data_ptr(), ldw,
+                  s.data_ptr(), K, N, S, out.data_ptr(), ldy, work.data_ptr() if size else None, size)
     return None if rc == L.DECLINED else out
 
 
@@ -618,7 +670,7 @@ def qkv_proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, q_gamma: torch.Tensor | 
     normalise the bf16 product, as qkv_proj() does; ROUND_ONCE keeps it in fp32 up to the one
     rounding of Q and K. Returns (q, k, v) as [heads, seq_pad, head_dim] bf16, or None when the
     geometry is declined."""
-    x, device, S, n, N, ldx, ldw = _mx4_product(x, w)
+    device, S, N, ldx, ldw = _mx4_operands(x, w)
     if N != 3 * heads * head_dim:
         raise ValueError(f"w must hold [{3 * heads * head_dim}, {w.cols}], got {w.shape}")
     seq_pad = seq_pad or (S + L.TILE - 1) // L.TILE * L.TILE
@@ -634,20 +686,33 @@ def qkv_proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, q_gamma: torch.Tensor | 
         out = tuple(out)
         for t in out:
             _require_out(t, shape, device)
-    q_out, k_out, v_out = out
-    rc = _run(L.lib().h3hip_qkv_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
-              w.values.data_ptr(), ldw, w.scale.data_ptr(), 2 * n, gq, gk, eps, tab, rot, rounding,
-              S, seq_pad, heads, head_dim, q_out.data_ptr(), k_out.data_ptr(), v_out.data_ptr())
+    q, k, o = out
+    v, s, K = w
+    norm = (gq, gk, eps, tab, rot, rounding, S, seq_pad, heads, head_dim, q.data_ptr(),
+            k.data_ptr(), o.data_ptr())
+    if type(x) is Mx4Rows:
+        rc = _run(L.lib().h3hip_qkv_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
+                  v.data_ptr(), ldw, s.data_ptr(), 2 * v.shape[1], *norm)
+    else:
+        size, work = _mx4_workspace(S, K, heads), None
+        if size:
+            work = _empty(size, dtype=_U8, device=device)
+        rc = _run(L.lib().h3hip_qkv_linear_mx4, device, x.data_ptr(), ldx, v.data_ptr(), ldw,
+                  s.data_ptr(), K, *norm, work.data_ptr() if size else None, size)
     return None if rc == L.DECLINED else out
 
 
 # -------------------------------------- norm, modulation, gate and residual
 
-def _norm_rows(name: str, t: torch.Tensor, shape, device) -> int:
+def _norm_rows(name: str, t: torch.Tensor, S: int, hidden: int, device) -> int:
     """Checks bf16 rows of a norm; returns their stride."""
+    if t.dtype is _BF16 and t.device == device and t.shape == (S, hidden):
+        ld, step = t.stride()
+        if step == 1:
+            return ld if S > 1 else hidden
     ld = _rows(name, t, _BF16)
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    if t.shape != (S, hidden):
+        raise ValueError(f"{name} must be [{S}, {hidden}], got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
     return ld
@@ -665,19 +730,21 @@ def _norm_table(name: str, t, segments: int, hidden: int, device):
     """(address, row stride) of a modulation [segments, hidden] or, of one segment, [hidden]."""
     if t is None:
         return None, hidden
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    if (t.dtype is not _BF16 or t.shape != (segments, hidden) or t.device != device
-            or (t.stride(1) != 1 and hidden > 1)):
-        raise ValueError(f"{name} must be bfloat16 [{segments}, {hidden}] on {device} with unit "
-                         f"column stride, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr(), (t.stride(0) if segments > 1 else hidden)
+    if (t.dtype is _BF16 and t.device == device
+            and (t.shape == (segments, hidden) or (segments == 1 and t.shape == (hidden,)))
+            and (t.stride(-1) == 1 or hidden == 1)):
+        return t.data_ptr(), (t.stride(0) if segments > 1 else hidden)
+    raise ValueError(f"{name} must be bfloat16 [{segments}, {hidden}] on {device} with unit column "
+                     f"stride, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _norm_c(gamma, scale, shift, segments, hidden, device) -> L.NormC:
     scale, ld_scale = _norm_table("scale", scale, segments, hidden, device)
     shift, ld_shift = _norm_table("shift", shift, segments, hidden, device)
     return L.NormC(_norm_gamma("gamma", gamma, hidden, device), scale, shift, ld_scale, ld_shift)
+
+
+_Starts = [ctypes.c_int32 * n for n in range(17)]
 
 
 def _segments(starts):
@@ -687,21 +754,9 @@ def _segments(starts):
     n = len(starts)
     if not 1 <= n <= 16:
         raise ValueError(f"segments must be 1 to 16 first rows, got {n}")
-    if any(not 0 <= int(v) <= _INT32_MAX for v in starts):
+    if min(starts) < 0 or max(starts) > _INT32_MAX:
         raise ValueError(f"segments must be rows from 0 to below 2^31, got {list(starts)}")
-    return (ctypes.c_int32 * n)(*map(int, starts)), n
-
-
-def _norm_input(x: torch.Tensor):
-    ld = _rows("x", x, _BF16)
-    S, hidden = x.shape
-    if hidden == 0:
-        raise ValueError("x must be [S, hidden > 0]")
-    if S > _INT32_MAX or hidden > _INT32_MAX:
-        _require_int32("x", x)
-    if not x.is_cuda:
-        raise ValueError("x must be a GPU tensor (no host fallback exists)")
-    return ld, S, hidden, x.device
+    return _Starts[n](*starts), n
 
 
 def norm_modulate(x: torch.Tensor, gamma: torch.Tensor | None = None,
@@ -713,13 +768,13 @@ def norm_modulate(x: torch.Tensor, gamma: torch.Tensor | None = None,
     (or [hidden], of one segment), each optional. segments: the first row of each, not
     descending, from 0 on (None: one segment). Returns h [S, hidden] bf16 (or writes ``out``, any
     row stride; x itself is allowed), or None when declined (hidden above 16,384)."""
-    ldx, S, hidden, device = _norm_input(x)
+    ldx, S, hidden, device = _bf16_rows(x)
     starts, n = _segments(segments)
     norm = _norm_c(gamma, scale, shift, n, hidden, device)
     if out is None:
         out, ldh = _empty(S, hidden, dtype=_BF16, device=device), hidden
     else:
-        ldh = _norm_rows("out", out, (S, hidden), device)
+        ldh = _norm_rows("out", out, S, hidden, device)
     rc = _run(L.lib().h3hip_norm_modulate, device, x.data_ptr(), ldx, S, hidden, norm, eps, starts,
               n, out.data_ptr(), ldh)
     return None if rc == L.DECLINED else out
@@ -737,8 +792,8 @@ def gated_residual(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None =
     before r is rounded. Returns r, with next_norm (r, h), [S, hidden] bf16 each, or None when
     declined (hidden above 16,384). ``out`` is r, or (r, h), to write into: any row stride, x or
     y themselves are allowed."""
-    ldx, S, hidden, device = _norm_input(x)
-    ldy = _norm_rows("y", y, (S, hidden), device)
+    ldx, S, hidden, device = _bf16_rows(x)
+    ldy = _norm_rows("y", y, S, hidden, device)
     starts, n = _segments(segments)
     gate, ld_gate = _norm_table("gate", gate, n, hidden, device)
     post = _norm_gamma("post_gamma", post_gamma, hidden, device)
@@ -756,9 +811,9 @@ def gated_residual(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None =
             h = _empty(S, hidden, dtype=_BF16, device=device)
     else:
         r, h = out if norm is not None else (out, None)
-        ldr = _norm_rows("out", r, (S, hidden), device)
+        ldr = _norm_rows("out", r, S, hidden, device)
         if h is not None:
-            ldh = _norm_rows("out[1]", h, (S, hidden), device)
+            ldh = _norm_rows("out[1]", h, S, hidden, device)
     rc = _run(L.lib().h3hip_gated_residual, device, x.data_ptr(), ldx, y.data_ptr(), ldy, S, hidden,
               gate, ld_gate, post, residual_scale, norm, eps, starts, n, r.data_ptr(), ldr,
               None if h is None else h.data_ptr(), ldh)

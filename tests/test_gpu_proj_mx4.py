@@ -133,7 +133,27 @@ def test_bf16_rows_are_rounded_on_the_way(h3, S, K, N):
     assert (bits16(ops.proj_mx4(xs, w)) == bits16(y)).all()
 
 
-@pytest.mark.parametrize("S", [1, 9, 16, 17, 40, 400])
+@pytest.mark.parametrize("S", [1, 2, 3])
+@pytest.mark.parametrize("K,N", [(8, 5), (256, 16), (264, 17), (1000, 300), (2560, 33), (5120, 40),
+                                 (6000, 31), (9984, 100), (10240, 16), (10248, 48), (20480, 20),
+                                 (30000, 18), (61000, 7), (100_000, 3)])
+def test_one_and_two_bf16_rows(h3, S, K, N):
+    """Every number of units in flight, whole and part batches, and the sizes that take the other
+    way: against the product of the rows' 4-bit form in 64 bits; nothing else is written."""
+    from h3hip import ops
+    g = torch.Generator(device="cuda")
+    g.manual_seed(S + K)
+    x = (torch.randn((S, K), generator=g, device="cuda") * torch.exp(
+        torch.randn((S, K), generator=g, device="cuda"))).to(torch.bfloat16)
+    w = mx4_operand(N, K, N, -8, 16)
+    buf = torch.full((S + 1, N + 3), 7.0, dtype=torch.bfloat16, device="cuda")
+    note(f"proj_mx4 of {S} bf16 rows K={K} N={N}")
+    y = ops.proj_mx4(x, w, out=buf[:S, :N])
+    check_product(y, ops.quant_rows_mx4(x), w)
+    assert (buf[S] == 7.0).all() and (buf[:, N:] == 7.0).all()
+
+
+@pytest.mark.parametrize("S", [1, 2, 9, 16, 17, 40, 400])
 def test_bf16_rows_that_are_not_finite(h3, S):
     from h3hip import ops
     g = torch.Generator(device="cuda")

@@ -83,7 +83,7 @@ def test_wrappers(h3):
     x = torch.zeros((4, 100), dtype=torch.bfloat16)
     for call in (ops.norm_modulate, lambda t: ops.gated_residual(t, t)):
         for t, word in ((x, "GPU"), (x.float(), "bfloat16"), (x.t(), "unit column stride"),
-                        (x[0], "2-D"), (x[:, :0], "hidden > 0")):
+                        (x[0], "2-D"), (x[:, :0], "K > 0")):
             with pytest.raises(ValueError, match=word):
                 call(t)
     wide = torch.empty((1, 2 ** 31), dtype=torch.bfloat16, device="meta")
