@@ -27,28 +27,30 @@ enum class ProjMx4Tile {   // channels x tokens; p: two workgroups a CU
   kNone,
 };
 
-// Microseconds of a launch: start + rounds * (tile + step * reduction steps), rounds
-// being the tiles the busiest CU runs.
+// Microseconds of a launch: start + rounds * (round + round_step * reduction steps) + share *
+// (tile + tile_step * steps), rounds being the tiles the busiest CU runs and share all tiles over
+// the CUs: what a CU waits for goes by rounds, what all of them share, the power limit and the
+// caches, by share.
 struct ProjMx4Shape {
   ProjMx4Tile tile;
   int channels, tokens;
-  float start, per_tile, per_step;
+  float start, round, round_step, per_tile, tile_step;
 };
 constexpr ProjMx4Shape kProjMx4Shapes[] = {
-    {ProjMx4Tile::k256x256, 256, 256, 0.0f, 12.0f, 1.04f},
-    {ProjMx4Tile::k256x224, 256, 224, 0.0f, 10.9f, 0.94f},
-    {ProjMx4Tile::k256x192, 256, 192, 0.1f, 9.5f, 0.83f},
-    {ProjMx4Tile::k256x160, 256, 160, 0.5f, 8.7f, 0.72f},
-    {ProjMx4Tile::k256x128, 256, 128, 0.8f, 7.2f, 0.63f},
-    {ProjMx4Tile::k128x192, 128, 192, 1.1f, 6.0f, 0.50f},
-    {ProjMx4Tile::k128x160, 128, 160, 1.5f, 5.1f, 0.46f},
-    {ProjMx4Tile::k128x128, 128, 128, 1.8f, 4.3f, 0.42f},
-    {ProjMx4Tile::k128x128p, 128, 128, 4.7f, 1.1f, 0.51f},
-    {ProjMx4Tile::k128x64p, 128, 64, 3.2f, 1.3f, 0.29f},
-    {ProjMx4Tile::k128x32p, 128, 32, 3.2f, 1.2f, 0.24f},
-    {ProjMx4Tile::k64x64p, 64, 64, 3.2f, 1.3f, 0.18f},
-    {ProjMx4Tile::k32x64p, 32, 64, 3.1f, 1.0f, 0.125f},
-    {ProjMx4Tile::k32x32p, 32, 32, 3.2f, 0.8f, 0.080f},
+    {ProjMx4Tile::k256x256, 256, 256, 4.56f, 4.45f, 0.965f, 6.75f, 0.632f},
+    {ProjMx4Tile::k256x224, 256, 224, 5.17f, 3.29f, 0.869f, 6.00f, 0.447f},
+    {ProjMx4Tile::k256x192, 256, 192, 4.46f, 3.04f, 0.727f, 5.55f, 0.405f},
+    {ProjMx4Tile::k256x160, 256, 160, 3.79f, 2.70f, 0.712f, 4.62f, 0.337f},
+    {ProjMx4Tile::k256x128, 256, 128, 4.36f, 3.27f, 0.615f, 3.55f, 0.245f},
+    {ProjMx4Tile::k128x192, 128, 192, 2.80f, 3.03f, 0.609f, 2.63f, 0.312f},
+    {ProjMx4Tile::k128x160, 128, 160, 2.83f, 2.91f, 0.384f, 2.34f, 0.264f},
+    {ProjMx4Tile::k128x128, 128, 128, 2.46f, 2.67f, 0.261f, 1.93f, 0.219f},
+    {ProjMx4Tile::k128x128p, 128, 128, 4.31f, 0.00f, 0.393f, 2.61f, 0.109f},
+    {ProjMx4Tile::k128x64p, 128, 64, 3.69f, 0.00f, 0.237f, 1.64f, 0.093f},
+    {ProjMx4Tile::k128x32p, 128, 32, 3.56f, 0.00f, 0.196f, 1.05f, 0.024f},
+    {ProjMx4Tile::k64x64p, 64, 64, 2.44f, 0.91f, 0.179f, 0.50f, 0.052f},
+    {ProjMx4Tile::k32x64p, 32, 64, 2.13f, 1.19f, 0.176f, 0.27f, 0.001f},
+    {ProjMx4Tile::k32x32p, 32, 32, 2.45f, 0.63f, 0.088f, 0.42f, 0.000f},
 };
 
 // Whether a shape's tiles can be counted and launched: 16 bits each way in a tile's
@@ -66,30 +68,35 @@ inline ProjGrid proj_mx4_grid(int tokens, int channels, int tile_tokens, int til
   return proj_grid(tokens, n * tile_channels, tile_tokens, tile_channels);
 }
 
+// Time of a launch of `tiles` tiles in `rounds` rounds.
+inline float proj_mx4_cost(const ProjMx4Shape& s, int tiles, int rounds, int steps) {
+  return s.start + (float)rounds * (s.round + s.round_step * (float)steps) +
+         (float)tiles / (32 * kOrderXcds) * (s.per_tile + s.tile_step * (float)steps);
+}
+
 // The shape whose launch takes least; kNone if none fits one. heads: the output is
-// written by heads, so a tile holds whole ones.
+// written by heads, so a tile holds whole ones. steps: of 256 values of the reduction.
 //
-// The constants are least squares over 440 sizes (1 to 18,102 tokens, 777 to 15,360
-// channels, 3 to 56 steps, without norm) of every shape on MI355X, whose times they give to
-// 9-19% (rms). What they pick is within 0.9% of the fastest shape on average, 15% at most, and
-// within 1.4-2.4% (31%) on 1,074 sizes of the QKV forms, which they were not fitted to. They
-// rank shapes and are no time of a call: neither the norm nor W's bytes are in them (QKV of
-// 1,151 x 56 heads x 5,376 is 89 us by them and takes 116-120). Few
-// rows are where it matters: one token x 5,120 x 5,120 takes 7.5 us on 160 tiles of 32 x 32,
-// 15.7 on 40 of 128 x 64 and 27 on 20 of 256 x 128; 125 tokens 12.7 on 64 x 64, 15.4 on 32 x 32.
+// The constants were fitted to what they pick: 7,571 sizes of both forms (1 to 32,000 tokens, 200 to
+// 21,504 channels, 1 to 28 steps; heads with norm in H3HIP_ROUND_ONCE) timed on every shape on MI355X.
+// On the 30% of them that the search did not see the pick is 1.2% slower than the best shape on
+// average; with a term in rounds alone, as for int8, whose constants lose 1.6% (3.8% past 2,000
+// tokens), least squares lose 1.7%. Every shape is the pick for 30 of the sizes or more, and
+// without it those take 3-20% longer. 31,885 tokens x 5,120 x 5,120 take 431 us on 256 x 192, 468
+// on 256 x 256 and 538 on 128 x 192; 1,151 x 56 heads x 5,376 77 us on 256 x 192, 88 on 256 x 256.
 inline ProjMx4Tile pick_proj_mx4_tile(int tokens, int channels, int steps, bool heads) {
   float best = 0.f;
   ProjMx4Tile tile = ProjMx4Tile::kNone;
   for (const ProjMx4Shape& s : kProjMx4Shapes) {
     if ((heads && s.channels < 128) || !proj_mx4_fits(tokens, channels, s)) continue;
-    const float round = s.per_tile + s.per_step * (float)steps;
     // A round for each tile a CU gets at least: most shapes need no look at their lists.
     const int tiles_m = (int)(((int64_t)tokens + s.tokens - 1) / s.tokens);
     const int tiles_n = (int)(((int64_t)channels + s.channels - 1) / s.channels);
-    const int least = (tiles_m * tiles_n + 32 * kOrderXcds - 1) / (32 * kOrderXcds);
-    if (tile != ProjMx4Tile::kNone && s.start + (float)least * round >= best) continue;
+    const int tiles = tiles_m * tiles_n;
+    const int least = (tiles + 32 * kOrderXcds - 1) / (32 * kOrderXcds);
+    if (tile != ProjMx4Tile::kNone && proj_mx4_cost(s, tiles, least, steps) >= best) continue;
     const int rounds = proj_mx4_grid(tokens, channels, s.tokens, s.channels).rounds;
-    const float cost = s.start + (float)rounds * round;
+    const float cost = proj_mx4_cost(s, tiles, rounds, steps);
     if (tile == ProjMx4Tile::kNone || cost < best) {
       best = cost;
       tile = s.tile;

@@ -9,6 +9,13 @@ from _mx4 import bits16, check_exact, check_product, decode64, mx4_operand, prod
 
 pytestmark = pytest.mark.gpu
 
+# One size for each tile shape (rows, in, out), with rows and channels that end inside a tile;
+# test_proj_mx4_tile_host.py checks which shape each one takes.
+SHAPES = [("256x256", 3001, 768, 5000), ("256x224", 4000, 512, 3500), ("256x192", 1301, 256, 9000),
+          ("256x160", 4000, 256, 2500), ("256x128", 641, 3584, 9000), ("128x192", 1700, 1024, 3500),
+          ("128x160", 3001, 768, 1300), ("128x128", 385, 1792, 5000), ("128x128p", 201, 256, 12000),
+          ("128x64p", 100, 256, 9000), ("128x32p", 65, 256, 9000), ("64x64p", 1, 256, 9000),
+          ("32x64p", 33, 256, 5000), ("32x32p", 1, 256, 100)]
 SIZES = [(1, 256, 1), (1, 32, 16), (1, 5120, 5120), (2, 256, 17), (7, 31, 33), (15, 512, 128),
          (16, 768, 130), (17, 768, 33), (31, 1280, 127), (33, 256, 777), (64, 2304, 512),
          (65, 4096, 129), (125, 5120, 5120), (129, 512, 640), (130, 1280, 256), (255, 1792, 1000),
@@ -26,6 +33,20 @@ def test_exact_sums(h3, S, K, N):
     torch.cuda.synchronize()
     assert y.shape == (S, N) and y.dtype == torch.bfloat16
     check_exact(y, product64(x, w))
+
+
+@pytest.mark.parametrize("shape,S,K,N", SHAPES, ids=[s[0] for s in SHAPES])
+def test_every_tile_shape(h3, shape, S, K, N):
+    """Into rows that are and are not on 16 bytes; nothing past a row's channels or the last row
+    is written. The reduction one block short of its last step, too."""
+    from h3hip import ops
+    for k, ldy, first in ((K, N + 8 - N % 8, 0), (K - 32, N + 3, 1)):
+        x, w = mx4_operand(S, k, S + k), mx4_operand(N, k, S + N)
+        buf = torch.full(((S + 1) * ldy + first,), 7.0, dtype=torch.bfloat16, device="cuda")
+        rows = buf[first:].view(S + 1, ldy)
+        note(f"proj_mx4 {shape} S={S} K={k} N={N} ldy={ldy}")
+        check_exact(ops.proj_mx4(x, w, out=rows[:S, :N]), product64(x, w))
+        assert (rows[S] == 7.0).all() and (rows[:, N:] == 7.0).all() and (buf[:first] == 7.0).all()
 
 
 @pytest.mark.parametrize("S,K,N", [(1, 5120, 300), (40, 2304, 512), (300, 1280, 1000),

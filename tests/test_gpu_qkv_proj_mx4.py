@@ -20,11 +20,21 @@ pytestmark = pytest.mark.gpu
 
 ONCE = 3
 
-CASES = [(1000, 768, 40, 128), (801, 512, 40, 96), (641, 768, 40, 96), (1000, 512, 24, 128),
-         (385, 768, 40, 96), (500, 256, 24, 96), (257, 256, 40, 128), (129, 1280, 40, 96),
-         (129, 256, 40, 128), (65, 256, 40, 96), (1, 256, 1, 96),
-         (900, 768, 39, 128), (2500, 512, 13, 96), (650, 768, 39, 96), (900, 512, 25, 128),
-         (385, 768, 41, 96), (4000, 512, 1, 128),
+# One size for each tile shape (rows, hidden, heads, rot); test_proj_mx4_tile_host.py
+# checks which shape each one takes.
+SHAPES = [("256x256", 1000, 768, 40, 128), ("256x224", 641, 256, 45, 96),
+          ("256x192", 1301, 256, 24, 128), ("256x160", 385, 256, 48, 96),
+          ("256x128", 201, 5120, 43, 128), ("128x192", 1301, 512, 12, 96),
+          ("128x160", 257, 512, 36, 128), ("128x128", 100, 1792, 43, 96),
+          ("128x128p", 201, 256, 31, 128), ("128x64p", 33, 256, 36, 96), ("128x32p", 1, 256, 1, 128)]
+# Odd head counts on tiles of 256 channels: the tiles between Q and K and between K and V
+# hold a head of each, the last one a single head.
+ODD_HEADS = [(1000, 768, 41, 128), (641, 256, 45, 96), (1301, 512, 23, 128), (385, 256, 49, 96),
+             (201, 5120, 43, 128)]
+CASES = [s[1:] for s in SHAPES] + ODD_HEADS
+CASES += [(1000, 768, 40, 96), (641, 512, 45, 128), (1301, 256, 24, 96), (385, 256, 48, 128),
+          (201, 5120, 43, 96), (1301, 512, 12, 128), (257, 512, 36, 96), (100, 1792, 43, 128),
+          (201, 256, 31, 96), (33, 256, 36, 128), (1, 256, 1, 96), (650, 768, 39, 96), (4000, 512, 1, 128),
          (1, 256, 1, 128), (1, 5120, 40, 128), (5, 512, 3, 96), (16, 768, 2, 128),
          (17, 1280, 2, 96), (33, 256, 5, 128), (65, 2304, 4, 96), (128, 512, 1, 96),
          (129, 1000, 4, 128), (300, 2048, 7, 128), (637, 5120, 40, 128), (1151, 5376, 56, 96),
