@@ -21,6 +21,11 @@ With ``projection="int8"`` both projections run on int8 operands with scales for
 each token and output channel (h3hip_quant_rows, h3hip_qkv_proj_i8,
 h3hip_proj_i8): the weights are rounded once, the activations in every call. A
 RopeState of ROUND_ONCE keeps Q and K in fp32 from that product to their store.
+``projection="mx4"`` is the same on microscaled 4-bit operands (h3hip_linear_mx4,
+h3hip_qkv_linear_mx4), a power of two for every 32 values of a row.
+
+AttentionBlock puts the layer between the norms of its DiT block: norm and modulation before
+(h3hip_norm_modulate), post-norm, gate and residual after (h3hip_gated_residual).
 """
 from __future__ import annotations
 
@@ -95,13 +100,14 @@ class AttentionLayer:
     when its kernel declines the geometry. "int8" runs both projections on int8
     operands (qkv_weight and out_weight are rounded here, or given as Int8Weight;
     the bf16 ones are not kept, so nothing is fallen back to), of at most
-    ops.INT8_MAX_REDUCTION in features, padded to a multiple of 128."""
+    ops.INT8_MAX_REDUCTION in features, padded to a multiple of 128. "mx4" runs both on 4-bit
+    operands in the same way (given as ops.Mx4Rows, or rounded here)."""
 
     def __init__(self, qkv_weight, out_weight, q_gamma, k_gamma, *, heads: int,
                  head_dim: int = 128, eps: float = 1e-5, backend: H3AttentionBackend | None = None,
                  projection: str = "hipblaslt"):
-        if projection not in ("fused", "hipblaslt", "int8"):
-            raise ValueError("projection must be 'fused', 'hipblaslt' or 'int8', got "
+        if projection not in ("fused", "hipblaslt", "int8", "mx4"):
+            raise ValueError("projection must be 'fused', 'hipblaslt', 'int8' or 'mx4', got "
                              f"{projection!r}")
         inner = heads * head_dim
         if qkv_weight.shape[0] != 3 * inner or out_weight.shape[1] != inner:
@@ -116,6 +122,11 @@ class AttentionLayer:
                                       for w in (qkv_weight, out_weight))
         elif isinstance(qkv_weight, Int8Weight) or isinstance(out_weight, Int8Weight):
             raise ValueError("an Int8Weight needs projection='int8'")
+        if projection == "mx4":
+            qkv_weight, out_weight = (w if isinstance(w, ops.Mx4Rows) else ops.quant_rows_mx4(w)
+                                      for w in (qkv_weight, out_weight))
+        elif isinstance(qkv_weight, ops.Mx4Rows) or isinstance(out_weight, ops.Mx4Rows):
+            raise ValueError("Mx4Rows as weights need projection='mx4'")
         self.qkv_weight, self.out_weight = qkv_weight, out_weight
         self.q_gamma, self.k_gamma = q_gamma, k_gamma
         self.heads, self.head_dim, self.eps = heads, head_dim, eps
@@ -152,6 +163,12 @@ class AttentionLayer:
                             seq_pad=seq_pad, rounding=rope.rounding)
         return None if r is None else tuple(t[:, :S] for t in r)
 
+    def _project_mx4(self, x, rope: RopeState, seq_pad: int):
+        r = ops.qkv_proj_mx4(x, self.qkv_weight, self.q_gamma, self.k_gamma, rope.table,
+                             heads=self.heads, head_dim=self.head_dim, eps=self.eps,
+                             seq_pad=seq_pad, rounding=rope.rounding)
+        return None if r is None else tuple(t[:, :x.shape[0]] for t in r)
+
     def _attend(self, q, k, v, context: AttentionContext | None):
         """AttentionLayer.sdpa (DiTBlock.swift:280-328) on [H, S, D] views:
         the backend only with a context; a decline runs dense SDPA."""
@@ -181,14 +198,15 @@ class AttentionLayer:
             raise ValueError(f"x must be [S, {self.qkv_weight.shape[1]}] (the packed-row layout), "
                              f"got {tuple(x.shape)}")
         S = x.shape[0]
-        if rope is not None and rope.rounding == L.ROUND_ONCE and self.projection != "int8":
-            raise ValueError("ROUND_ONCE needs projection='int8'")
+        if (rope is not None and rope.rounding == L.ROUND_ONCE
+                and self.projection not in ("int8", "mx4")):
+            raise ValueError("ROUND_ONCE needs projection='int8' or 'mx4'")
         if rope is None:
             rope = RopeState.identity(S, self.head_dim, x.device)
         seq_pad = ((S + L.TILE - 1) // L.TILE) * L.TILE
         paths = {"fused": (self._project_fused, self._project_hipblaslt),
                  "hipblaslt": (self._project_hipblaslt, self._project_fused),
-                 "int8": (self._project_int8,)}[self.projection]
+                 "int8": (self._project_int8,), "mx4": (self._project_mx4,)}[self.projection]
         qkv = None
         for project in paths:
             qkv = qkv or project(x, rope, seq_pad)
@@ -199,7 +217,58 @@ class AttentionLayer:
         if self.projection == "int8":
             return ops.proj_i8(*ops.quant_rows(merged), self.out_weight.values,
                                self.out_weight.scale)
+        if self.projection == "mx4":
+            return ops.proj_mx4(merged, self.out_weight)
         y = ops.out_proj(merged, self.out_weight)
         if y is None:       # a width the kernel declines: hipBLASLt's GEMM
             y = torch.mm(merged, self.out_weight.t())
         return y
+
+
+@dataclass
+class Modulation:
+    """What a timestep's conditioning makes of a block's attention half: tables
+    [segments, hidden] bf16 (or [hidden], of one segment), each optional."""
+    scale: torch.Tensor | None = None
+    shift: torch.Tensor | None = None
+    gate: torch.Tensor | None = None
+
+
+class AttentionBlock:
+    """The attention half of a DiT block around an AttentionLayer:
+
+        h = norm(x; gamma) (1 + scale[s]) + shift[s]
+        r = residual_scale x + gate[s] z,  z = layer(h) or norm(layer(h); post_gamma)
+
+    for a residual stream x [S, hidden], s being a token's segment (text, audio and video are
+    modulated apart: ``segments`` holds the first row of each). The norms are over the hidden
+    width, in one kernel each with what follows them (h3hip_norm_modulate,
+    h3hip_gated_residual); widths above 16,384 are refused when the block is made."""
+
+    def __init__(self, layer: AttentionLayer, gamma: torch.Tensor | None = None,
+                 post_gamma: torch.Tensor | None = None, *, residual_scale: float = 1.0,
+                 eps: float = 1e-6):
+        hidden = layer.qkv_weight.shape[1]
+        if layer.out_weight.shape[0] != hidden:
+            raise ValueError(f"a residual needs {hidden} out features, the layer has "
+                             f"{layer.out_weight.shape[0]}")
+        if hidden > ops.NORM_MAX_HIDDEN:
+            raise NotImplementedError(f"no norm kernel takes a hidden width of {hidden} (at most "
+                                      f"{ops.NORM_MAX_HIDDEN})")
+        self.layer, self.gamma, self.post_gamma = layer, gamma, post_gamma
+        self.residual_scale, self.eps = residual_scale, eps
+
+    def __call__(self, x: torch.Tensor, rope: RopeState | None,
+                 context: AttentionContext | None = None, modulation: Modulation | None = None, *,
+                 segments=None, normed: torch.Tensor | None = None, next_norm: dict | None = None):
+        """x: [S, hidden] bf16 -> r [S, hidden] bf16, with next_norm (r, h): h is the norm that
+        the next half begins with (a dict of its gamma, scale and shift), which that half then
+        takes as its ``normed`` instead of norming r itself."""
+        m = modulation or Modulation()
+        if normed is None:
+            normed = ops.norm_modulate(x, self.gamma, m.scale, m.shift, segments=segments,
+                                       eps=self.eps)
+        y = self.layer(normed, rope, context)
+        return ops.gated_residual(x, y, m.gate, post_gamma=self.post_gamma,
+                                  residual_scale=self.residual_scale, segments=segments,
+                                  eps=self.eps, next_norm=next_norm)

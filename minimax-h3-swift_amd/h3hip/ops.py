@@ -704,6 +704,9 @@ def qkv_proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, q_gamma: torch.Tensor | 
 
 # -------------------------------------- norm, modulation, gate and residual
 
+NORM_MAX_HIDDEN = 16384          # widths that a workgroup's registers hold
+
+
 def _norm_rows(name: str, t: torch.Tensor, S: int, hidden: int, device) -> int:
     """Checks bf16 rows of a norm; returns their stride."""
     if t.dtype is _BF16 and t.device == device and t.shape == (S, hidden):
