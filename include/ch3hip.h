@@ -395,8 +395,8 @@ int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const vo
                        int32_t head_dim, void* q_out, void* k_out, void* v_out, void* stream);
 
 /* h3hip_proj_mx4 of bf16 rows, which are rounded as by h3hip_quant_rows_mx4 on the way: in a launch
- * of their own before the product, or of one or two rows (of a multiple of 8 columns) in the
- * same launch, whose sums add in another order.
+ * of their own before the product, or, one or two rows (of a multiple of 8 columns), in the
+ * product's launch, whose sums add in another order.
  *   x: device bf16 [rows, in_features], row stride ldx elements; rows may begin anywhere; any
  *      in_features (up to 33,553,920). w, w_scale: rows of in_features columns as
  *      h3hip_quant_rows_mx4 writes them (padded to a multiple of 256, zeros). y as there.

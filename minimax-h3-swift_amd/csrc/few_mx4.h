@@ -1,7 +1,7 @@
-// Arguments of the 4-bit projection of one or two bf16 rows (few_mx4.hip) and its launch.
+// Arguments of the 4-bit projections of one or two bf16 rows (few_mx4.hip) and their launches.
 #pragma once
 
-#include "common.h"
+#include "proj.h"
 
 namespace h3hip {
 
@@ -9,7 +9,8 @@ struct FewMx4Args {
   const uint16_t* __restrict__ x;        // [rows, cols], row stride ldx elements
   const uint8_t* __restrict__ w;         // [n_total, units * 128], row stride ldw bytes
   const uint8_t* __restrict__ w_scale;
-  uint16_t* __restrict__ y;              // [rows, n_total], row stride ldy elements
+  uint16_t* __restrict__ y;              // [rows, n_total], row stride ldy elements, or
+  float* __restrict__ sums;              // [rows, n_total] where it is not NULL
   int64_t ldx, ldw, ldy;
   int32_t rows, cols, units, n_total;    // units: of 256 values of the reduction
 };
@@ -17,5 +18,8 @@ struct FewMx4Args {
 // Whether few_mx4_kernel takes a call of these sizes.
 bool few_mx4_takes(int32_t rows, int32_t cols);
 int launch_few_mx4(const FewMx4Args& a, hipStream_t stream);
+// Q, K and V of sums [seq_len, 3 * heads * 128] (16-byte aligned): out as in ProjMx4Args.
+int launch_few_heads(const float* sums, const ProjArgs& out, int32_t rounding, bool plain,
+                     hipStream_t stream);
 
 }  // namespace h3hip

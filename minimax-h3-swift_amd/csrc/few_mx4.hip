@@ -1,4 +1,4 @@
-// The 4-bit projection of one or two bf16 rows: their rounding and the product in one launch.
+// The 4-bit projections of one or two bf16 rows: their rounding and the product in one launch.
 //
 // What bounds it: W's bytes, 17/32 of one a value (5,120 x 5,120: 14 MB, 2.9 us at the rate of a
 // large copy), the launch and the latencies in a row of the rows' loads, W's and the store. So
@@ -8,10 +8,17 @@
 // 640 lanes' work). A wave takes every fourth 256 values of the reduction: A is 16 rows of W
 // straight from memory, B the rows' codes from LDS, in v_mfma_scale_f32_16x16x128_f8f6f4 as in
 // proj_mx4_kernel.h. The four sums are added in LDS, in one order.
+//
+// Of Q | K | V, whose head norm needs 128 channels at once, the sums go to a workspace in fp32, and
+// a second launch of a workgroup a head norms, rotates and stores them. Workgroups of whole heads
+// in one launch leave half the CUs idle, whose loads are what W takes: 13.7 us and more of one
+// token x 5,120 x 40 heads, as the tiles of 128 x 32 behind a rounding of their own do (13.4; of a
+// W that no cache holds 17.3).
 #include <algorithm>
 
 #include "few_mx4.h"
 #include "mx4_block.h"
+#include "proj_rows.h"
 
 namespace h3hip {
 
@@ -37,8 +44,8 @@ inline int64_t lds_bytes(int rows, int units, int hold) {
 constexpr int64_t kMaxLds = 65536;
 inline int hold_of(int units) { return std::min((units + kWaves - 1) / kWaves, kMaxHold); }
 
-// kHold units of a wave in flight.
-template <int kHold>
+// kHold units of a wave in flight; kSums: fp32 sums to a.sums instead of bf16 to a.y.
+template <int kHold, bool kSums>
 __global__ __launch_bounds__(kThreads) void few_mx4_kernel(FewMx4Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = (int)threadIdx.x, lane = tid & 63;
@@ -147,15 +154,74 @@ __global__ __launch_bounds__(kThreads) void few_mx4_kernel(FewMx4Args a) {
     float y = 0.f;
 #pragma unroll
     for (int s = 0; s < kWaves; s++) y += sums[(s * rows + r) * kSumStride + c];
-    if (n0 + c < a.n_total)
-      a.y[r * a.ldy + n0 + c] = (uint16_t)(pack_bf16x2(y, y) & 0xffffu);
+    if (n0 + c < a.n_total) {
+      if constexpr (kSums)
+        a.sums[r * (int64_t)a.n_total + n0 + c] = y;
+      else
+        a.y[r * a.ldy + n0 + c] = (uint16_t)(pack_bf16x2(y, y) & 0xffffu);
+    }
   }
+}
+
+// Sums [rows, 3 * heads * 128] in fp32 to the heads: a workgroup a head, 8 lanes a row in the
+// prologue's layout, and zeros into the rows behind the last. kPlain: no norm and rotation.
+template <int kMode, int kHl, bool kPlain>
+__global__ __launch_bounds__(kThreads) void few_heads_kernel(const float* __restrict__ sums,
+                                                             ProjArgs o) {
+  constexpr bool kFull = kHl == 8;
+  const int head = (int)blockIdx.x, part = head / o.heads;
+  const int row = (int)threadIdx.x >> 3, j = (int)threadIdx.x & 7;
+  if (row < o.seq_len) {
+    const bool pair_lane = kFull || j < kHl;
+    const int chunk_a = pair_lane ? j : 2 * kHl + 2 * (j - kHl);
+    const int chunk_b = pair_lane ? j + kHl : chunk_a + 1;
+    const float* src = sums + ((int64_t)row * 3 * o.heads + head) * 128;
+    float v[16];
+#pragma unroll
+    for (int h = 0; h < 4; h++) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(src + 8 * (h < 2 ? chunk_a : chunk_b) +
+                                                      4 * (h & 1));
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[4 * h + i] = t[i];
+    }
+    u32x4 oa = pack8(v), ob = pack8(v + 8);
+    if (!kPlain && part < 2) {
+      if (kMode != H3HIP_ROUND_ONCE) unpack8(oa, v), unpack8(ob, v + 8);   // of the bf16 product
+      float gam[16];
+      const uint16_t* gsrc = part == 0 ? o.q_gamma : o.k_gamma;
+      unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_a), gam);
+      unpack8(*reinterpret_cast<const u32x4*>(gsrc + 8 * chunk_b), gam + 8);
+      RopeEntry tab[8] = {};
+      if (pair_lane) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {      // entry 8j + i of the row: c, -s, s, c
+          const int64_t at = ((int64_t)row * 8 * kHl + 8 * j + i) * 4;
+          if (kMode == H3HIP_ROUND_REFERENCE) {
+            const u32x2 t = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(o.table) + at);
+            tab[i] = RopeEntry{bf16_lo(t[0]), bf16_lo(t[1])};
+          } else {
+            const f32x4 t = *reinterpret_cast<const f32x4*>(static_cast<const float*>(o.table) + at);
+            tab[i] = RopeEntry{t[0], t[2]};
+          }
+        }
+      }
+      norm_rope<kMode, kFull>(v, gam, pair_lane, tab, o.eps, oa, ob);
+    }
+    uint16_t* dst = head_rows(o, head) + (int64_t)row * 128;
+    *reinterpret_cast<u32x4*>(dst + 8 * chunk_a) = oa;
+    *reinterpret_cast<u32x4*>(dst + 8 * chunk_b) = ob;
+  }
+  zero_rows<128, kThreads>(o, (int)threadIdx.x, o.seq_len, 128 * head);
 }
 
 template <int kHold>
 void launch(const FewMx4Args& a, hipStream_t st) {
-  const unsigned grid = (unsigned)(((int64_t)a.n_total + kChannels - 1) / kChannels);
-  few_mx4_kernel<kHold><<<dim3(grid), kThreads, lds_bytes(a.rows, a.units, kHold), st>>>(a);
+  const dim3 grid((unsigned)(((int64_t)a.n_total + kChannels - 1) / kChannels));
+  const size_t lds = lds_bytes(a.rows, a.units, kHold);
+  if (a.sums)
+    few_mx4_kernel<kHold, true><<<grid, kThreads, lds, st>>>(a);
+  else
+    few_mx4_kernel<kHold, false><<<grid, kThreads, lds, st>>>(a);
 }
 
 }  // namespace
@@ -180,6 +246,28 @@ int launch_few_mx4(const FewMx4Args& a, hipStream_t st) {
     default: launch<kMaxHold>(a, st);
   }
   return check_launch("few_mx4_kernel");
+}
+
+int launch_few_heads(const float* sums, const ProjArgs& o, int32_t rounding, bool plain,
+                     hipStream_t st) {
+  constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32, kOnce = H3HIP_ROUND_ONCE;
+  const dim3 grid((unsigned)(3 * o.heads));
+  const bool full = o.rot == 128;
+  if (plain)
+    few_heads_kernel<kRef, 8, true><<<grid, kThreads, 0, st>>>(sums, o);
+  else if (rounding == kRef && full)
+    few_heads_kernel<kRef, 8, false><<<grid, kThreads, 0, st>>>(sums, o);
+  else if (rounding == kRef)
+    few_heads_kernel<kRef, 6, false><<<grid, kThreads, 0, st>>>(sums, o);
+  else if (rounding == kF32 && full)
+    few_heads_kernel<kF32, 8, false><<<grid, kThreads, 0, st>>>(sums, o);
+  else if (rounding == kF32)
+    few_heads_kernel<kF32, 6, false><<<grid, kThreads, 0, st>>>(sums, o);
+  else if (full)
+    few_heads_kernel<kOnce, 8, false><<<grid, kThreads, 0, st>>>(sums, o);
+  else
+    few_heads_kernel<kOnce, 6, false><<<grid, kThreads, 0, st>>>(sums, o);
+  return check_launch("few_heads_kernel");
 }
 
 }  // namespace h3hip

@@ -6,8 +6,8 @@
 // h3hip_proj_mx4 writes y token-major; h3hip_qkv_proj_mx4 treats it as Q | K | V heads and ends as
 // h3hip_qkv_proj_i8 does: Q and K are h3hip_qk_norm_rope of h3hip_proj_mx4's result, bit for bit,
 // or in H3HIP_ROUND_ONCE the norm and rotation of the fp32 sums. The linear forms take bf16 rows
-// and round them on the way, one or two in the same launch (few_mx4.hip), more, and heads', in
-// one before it.
+// and round them on the way, one or two in the product's launch (few_mx4.hip), more in one before
+// it.
 #include "few_mx4.h"
 #include "proj_mx4.h"
 
@@ -135,20 +135,24 @@ int product(const ProjArgs& o, const void* x, int64_t ldx, const void* x_scale, 
 // Bytes of the codes of `rows` rows in a workspace; their scales follow.
 int64_t code_bytes(int32_t rows, int32_t in) { return (int64_t)rows * (padded(in) / 2); }
 
-// The product of bf16 rows: one or two in one launch, more rounded into the workspace first.
+// The product of bf16 rows: one or two rounded on the way, more into the workspace first.
 int linear(const ProjArgs& o, const void* x, int64_t ldx, const void* w, int64_t ldw,
            const void* w_scale, int32_t in, int32_t n_total, int32_t rounding, bool plain, bool out,
            void* workspace, int64_t workspace_bytes, void* stream) {
-  if (out && few_mx4_takes(o.seq_len, in))
-    return launch_few_mx4(
-        FewMx4Args{static_cast<const uint16_t*>(x), static_cast<const uint8_t*>(w),
-                   static_cast<const uint8_t*>(w_scale), o.q_out, ldx, ldw, o.ldo, o.seq_len, in,
-                   (int32_t)(padded(in) / 256), n_total},
-        as_stream(stream));
   const int64_t need = h3hip_linear_mx4_workspace(o.seq_len, in, out ? 0 : o.heads);
-  H3_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), H3HIP_EINVAL,
-             "a workspace of %lld bytes, 16-byte aligned, is needed (%lld given)", (long long)need,
-             (long long)(workspace ? workspace_bytes : 0));
+  H3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
+             H3HIP_EINVAL, "a workspace of %lld bytes, 16-byte aligned, is needed (%lld given)",
+             (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  if (few_mx4_takes(o.seq_len, in)) {
+    float* sums = out ? nullptr : static_cast<float*>(workspace);
+    const int rc = launch_few_mx4(
+        FewMx4Args{static_cast<const uint16_t*>(x), static_cast<const uint8_t*>(w),
+                   static_cast<const uint8_t*>(w_scale), o.q_out, sums, ldx, ldw, o.ldo, o.seq_len,
+                   in, (int32_t)(padded(in) / 256), n_total},
+        as_stream(stream));
+    if (rc != H3HIP_OK || out) return rc;
+    return launch_few_heads(sums, o, rounding, plain, as_stream(stream));
+  }
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scale = codes + code_bytes(o.seq_len, in);
   const int64_t ld = padded(in) / 2;
@@ -208,7 +212,9 @@ extern "C" int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scal
 }
 
 extern "C" int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features, int32_t heads) {
-  if (rows <= 0 || in_features <= 0 || (heads == 0 && few_mx4_takes(rows, in_features))) return 0;
+  if (rows <= 0 || in_features <= 0) return 0;
+  if (few_mx4_takes(rows, in_features))
+    return heads > 0 ? (int64_t)rows * heads * (3 * kHeadDim * sizeof(float)) : 0;
   const int64_t slabs = ((int64_t)in_features + 511) / 512, groups = ((int64_t)rows + 15) / 16;
   return code_bytes(rows, in_features) + 256 * slabs * groups;
 }

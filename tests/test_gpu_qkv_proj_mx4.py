@@ -131,6 +131,32 @@ def test_bf16_rows_are_rounded_on_the_way(h3, S, K, H, rounding):
             assert (bits16(a) == bits16(b)).all()
 
 
+@pytest.mark.parametrize("S", [1, 2, 3])
+@pytest.mark.parametrize("K,H,rot", [(8, 1, 128), (264, 3, 96), (1000, 5, 128), (5376, 7, 96),
+                                     (10248, 2, 128)])
+def test_one_and_two_bf16_rows(h3, S, K, H, rot):
+    """Every rounding and the plain product, on whole numbers (exact sums): the bits of the 4-bit
+    form's call, whichever way the sums were added, and zeros up to a far seq_pad."""
+    from h3hip import ops
+    g = torch.Generator(device="cuda")
+    g.manual_seed(S + K)
+    x = torch.randint(-8, 9, (S, K), generator=g, device="cuda").to(torch.bfloat16)
+    w = mx4_operand(3 * H * D, K, H)
+    q, gammas = ops.quant_rows_mx4(x), _gammas(K)
+    size = product64(q._replace(values=q.values & 0x77), w._replace(values=w.values & 0x77))
+    assert float(4 * size.max()) < 2 ** 24      # any partial sum is exact in fp32
+    for rounding in (0, 1, ONCE):
+        args = (*gammas, _rope(S, rot, rounding)[3])
+        note(f"qkv_proj_mx4 of {S} bf16 rows K={K} H={H} rot={rot} rounding={rounding}")
+        out = [torch.full((H, 384, D), 9.0, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+        got = ops.qkv_proj_mx4(x, w, *args, heads=H, eps=EPS, rounding=rounding, out=out, seq_pad=384)
+        want = ops.qkv_proj_mx4(q, w, *args, heads=H, eps=EPS, rounding=rounding)
+        for a, b in zip(got, want):
+            assert (bits16(a[:, :128]) == bits16(b)).all() and not a[:, S:].any()
+    for a, b in zip(ops.qkv_proj_mx4(x, w, heads=H), ops.qkv_proj_mx4(q, w, heads=H)):
+        assert (bits16(a) == bits16(b)).all()
+
+
 @pytest.mark.parametrize("S,K,H", [(3, 512, 3), (300, 1280, 4), (1500, 512, 2)])
 def test_plain_product_head_major(h3, S, K, H):
     from h3hip import ops

@@ -4,6 +4,8 @@ them."""
 import os
 import re
 
+import pytest
+
 from test_codegen import CSRC, _asm, _counts
 
 FORMS = 6     # out-projection, plain QKV, and norm + RoPE in two roundings and two widths
@@ -44,7 +46,8 @@ def test_once_kernels_compiled_whole(tmp_path):
     assert _check(asm) == 22 and _mfmas(asm) > 0
 
 
-def test_rows_spill_nothing(tmp_path):
-    asm = _asm(tmp_path, "quant_mx4")
+@pytest.mark.parametrize("source", ["quant_mx4", "few_mx4"])
+def test_rows_spill_nothing(tmp_path, source):
+    asm = _asm(tmp_path, source)
     assert max(_counts(asm, "vgpr_spill_count")) == 0
     assert max(_counts(asm, "private_segment_fixed_size")) == 0

@@ -91,6 +91,58 @@ def test_qkv_proj(h3, bad, word):
     assert _qkv(h3, **bad) == _lib.EINVAL and word in h3.last_error()
 
 
+def _linear(h3, x=BUF, ldx=500, w=BUF, ldw=256, ws=BUF, k=500, n=64, rows=4, y=BUF, ldy=64, work=BUF,
+            size=1 << 20):
+    return h3.lib().h3hip_linear_mx4(x, ldx, w, ldw, ws, k, n, rows, y, ldy, work, size, None)
+
+
+def _qkv_linear(h3, x=BUF, ldx=500, w=BUF, ldw=256, ws=BUF, k=500, gq=BUF, gk=BUF, table=BUF, rot=128,
+                rounding=0, S=4, pad=128, H=2, D=128, q=BUF, ko=BUF, v=BUF, work=BUF, size=1 << 20):
+    return h3.lib().h3hip_qkv_linear_mx4(x, ldx, w, ldw, ws, k, gq, gk, 1e-6, table, rot, rounding,
+                                         S, pad, H, D, q, ko, v, work, size, None)
+
+
+LINEAR = [(dict(x=None), "NULL"), (dict(w=None), "NULL"), (dict(ws=None), "NULL"),
+          (dict(ldx=499), "ldx"), (dict(ldw=240), "ldw"), (dict(ldw=264), "ldw"),
+          (dict(x=at(1)), "aligned"), (dict(w=at(8)), "aligned"), (dict(ws=at(2)), "aligned"),
+          (dict(ldw=1 << 26), "2 GiB"), (dict(k=1 << 25, ldx=1 << 26, ldw=1 << 25), "2 GiB"),
+          (dict(work=None), "workspace"), (dict(work=at(8)), "workspace")]
+
+
+@pytest.mark.parametrize("bad,word", LINEAR + [
+    (dict(k=0), "shape"), (dict(n=0), "shape"), (dict(rows=-1), "shape"), (dict(y=None), "NULL"),
+    (dict(ldy=63), "ldy"), (dict(y=at(1)), "aligned"), (dict(size=4 * 256 + 255), "workspace")])
+def test_linear(h3, bad, word):
+    from h3hip import _lib
+    assert _linear(h3, **bad) == _lib.EINVAL and word in h3.last_error()
+
+
+@pytest.mark.parametrize("bad,word", LINEAR + [
+    (dict(k=0), "hidden"), (dict(S=0), "shape"), (dict(H=0), "shape"), (dict(pad=64), "shape"),
+    (dict(gq=None), "gammas"), (dict(table=None), "table"), (dict(rounding=2), "rounding"),
+    (dict(q=None), "NULL"), (dict(v=at(8)), "aligned"), (dict(size=4 * 256 + 255), "workspace"),
+    (dict(S=2, k=504, ldx=504, size=2 * 2 * 1536 - 1), "workspace")])
+def test_qkv_linear(h3, bad, word):
+    from h3hip import _lib
+    assert _qkv_linear(h3, **bad) == _lib.EINVAL and word in h3.last_error()
+
+
+def test_linear_workspace(h3):
+    """Codes and scales of the rows, or the sums of one or two rows' heads; none for their
+    token-major product, nor where there is nothing to do."""
+    from h3hip import _lib
+    size = h3.lib().h3hip_linear_mx4_workspace
+    assert size(4, 500, 0) == size(4, 500, 7) == 4 * 256 + 256
+    assert size(100, 5120, 0) == 100 * 2560 + 10 * 7 * 256
+    assert size(2, 504, 0) == 0 and size(2, 504, 3) == 2 * 3 * 384 * 4
+    assert size(2, 500, 0) == 2 * 256 + 256        # not a multiple of 8 columns
+    assert size(2, 200_000, 0) == 2 * 100_096 + 391 * 256    # codes past the LDS
+    assert size(0, 500, 0) == size(4, 0, 0) == size(-1, -1, -1) == 0
+    assert _linear(h3, rows=0, x=None, y=None, work=None, size=0) == _lib.OK
+    for bad in (dict(D=64), dict(rot=64)):
+        assert _qkv_linear(h3, **bad) == _lib.DECLINED and "declined" in h3.last_error()
+
+
 def _u8(*shape):
     return torch.zeros(shape, dtype=torch.uint8)
 
