@@ -9,10 +9,12 @@
 // fp32 between the loads and the one rounding of r and of h; h is normalised from the fp32 r, not
 // from the rounded one.
 //
-// Bound by HBM: before 4 bytes an element, after with a next norm 8. So a row is read once and
+// Bound by HBM: before 4 bytes an element, after with a next norm 8 (31,885 x 5,120: 137 us, 4.8
+// TB/s, and 265 us, 4.9; a copy of 1 GiB 5.1), of few rows by the launch (125 x 5,120: 4.2 us). So a row is read once and
 // stays in registers through its sums, and the tables, which as rows are as long as x's, are held
 // in registers too, by workers that take a range of consecutive rows each and reload the
-// tables only where a segment begins. The next row's loads are in flight while one is summed.
+// tables only where a segment begins. The next row's loads are in flight while one is summed (of
+// widths up to 8,192).
 // A worker is a workgroup of as many waves as the row has chunks of 512 elements (of 1,024 past
 // 8,192): 8 elements a thread. That depends on the width alone, and sums add in one order, so a
 // row's bits do not depend on the other rows of the call.
@@ -30,7 +32,9 @@ constexpr int kLaneElems = 8;              // consecutive elements of a thread i
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxHidden = 2 * kMaxThreads * kLaneElems;
 constexpr int kCus = 256;
-constexpr int kWavesCu = 28;               // what its registers leave room for
+// Waves a CU: 6 a SIMD in 80 registers. In the 94 that the compiler took by itself two workgroups of
+// 11 waves did not fit a CU (31,885 x 5,376, after with a next norm, 373 us; 290).
+constexpr int kWavesCu = 24;
 
 struct NormArgs {
   const uint16_t* x;                       // r or h may be x or y
@@ -58,9 +62,17 @@ __device__ __forceinline__ u32x4 load8(const uint16_t* row, int k, int n) {
   return v;
 }
 
+// kPast: past the caches, for what is not read again soon. r with a next norm's h beside it is: the
+// next half reads h at once and r at its end (both and the rounding of h to 4 bits at 1,151 x 5,376
+// 23.4 -> 22.2 us, 31,885 x 5,120 342 -> 339). h is not: stored past the caches it took 58 us
+// instead of 87 alone (18,102 x 5,120 again and again) and 136 instead of 117 with its rounding.
+template <bool kPast>
 __device__ __forceinline__ void store8(uint16_t* row, int k, int n, u32x4 v) {
   if (k + 8 <= n) {
-    *reinterpret_cast<u32x4_any*>(row + k) = v;
+    if constexpr (kPast)
+      __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(row + k));
+    else
+      *reinterpret_cast<u32x4_any*>(row + k) = v;
     return;
   }
 #pragma unroll
@@ -101,7 +113,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 // kChunks chunks of a row a thread. kAfter: there is y; kPost: it is normalised; kNext: h is
 // written (without kAfter always).
 template <int kChunks, bool kAfter, bool kPost, bool kNext>
-__global__ __launch_bounds__(kMaxThreads) void norm_residual_kernel(NormArgs a) {
+__global__ __launch_bounds__(kMaxThreads) __attribute__((amdgpu_waves_per_eu(kChunks == 1 ? 6 : 4)))
+void norm_residual_kernel(NormArgs a) {
   constexpr int kSums = (kPost ? 1 : 0) + (kNext ? 1 : 0);
   constexpr int kMaxWaves = kMaxThreads / 64;
   __shared__ __attribute__((aligned(16))) float part[2][kSums > 0 ? kSums : 1][kMaxWaves];
@@ -141,7 +154,8 @@ __global__ __launch_bounds__(kMaxThreads) void norm_residual_kernel(NormArgs a) 
       if constexpr (kAfter) ty[c] = load8(a.y + row * a.ldy, k, n);
     }
   };
-  load_row(first, vx, vy);
+  constexpr bool kAhead = kChunks == 1;    // two chunks a thread leave no registers for it
+  if (kAhead) load_row(first, vx, vy);
 
   // gate and post gamma in one factor, gamma and 1 + scale in one, and the shift, of the
   // row's segment.
@@ -187,7 +201,10 @@ __global__ __launch_bounds__(kMaxThreads) void norm_residual_kernel(NormArgs a) 
       load_tables(s);
     }
     u32x4 nx[kChunks], ny[kChunks];
-    if (row + 1 < last) load_row(row + 1, nx, ny);
+    if (!kAhead)
+      load_row(row, vx, vy);
+    else if (row + 1 < last)
+      load_row(row + 1, nx, ny);
     const int parity = (row - first) & 1;
 
     float v[kChunks][8];                   // x, then r
@@ -212,7 +229,7 @@ __global__ __launch_bounds__(kMaxThreads) void norm_residual_kernel(NormArgs a) 
         unpack(vy[c], t);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[c][i] = a.alpha * v[c][i] + fg[c][i] * (t[i] * rs);
-        store8(a.r + row * a.ldr, k0 + c * stride, n, pack(v[c]));
+        store8<kNext>(a.r + row * a.ldr, k0 + c * stride, n, pack(v[c]));
       }
     }
     if constexpr (kNext) {
@@ -227,13 +244,15 @@ __global__ __launch_bounds__(kMaxThreads) void norm_residual_kernel(NormArgs a) 
         float t[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) t[i] = v[c][i] * rs * fa[c][i] + fb[c][i];
-        store8(a.h + row * a.ldh, k0 + c * stride, n, pack(t));
+        store8<false>(a.h + row * a.ldh, k0 + c * stride, n, pack(t));
       }
     }
+    if constexpr (kAhead) {
 #pragma unroll
-    for (int c = 0; c < kChunks; c++) {
-      vx[c] = nx[c];
-      if constexpr (kAfter) vy[c] = ny[c];
+      for (int c = 0; c < kChunks; c++) {
+        vx[c] = nx[c];
+        if constexpr (kAfter) vy[c] = ny[c];
+      }
     }
   }
 }

@@ -51,3 +51,12 @@ def test_rows_spill_nothing(tmp_path, source):
     asm = _asm(tmp_path, source)
     assert max(_counts(asm, "vgpr_spill_count")) == 0
     assert max(_counts(asm, "private_segment_fixed_size")) == 0
+
+
+def test_norms_spill_nothing(tmp_path):
+    """And rows of one chunk a thread leave room for 24 waves a CU."""
+    asm = _asm(tmp_path, "norm_residual")
+    assert max(_counts(asm, "vgpr_spill_count")) == 0
+    assert max(_counts(asm, "private_segment_fixed_size")) == 0
+    vgpr = _counts(asm, "vgpr_count")
+    assert len(vgpr) == 10 and sorted(vgpr)[4] <= 80 and max(vgpr) <= 128, vgpr
