@@ -106,7 +106,7 @@ def test_wrapper_checks_of_tables(h3):
     for t in (good, good[0, :99], good[0].float(), torch.zeros(200, dtype=torch.bfloat16)[::2]):
         with pytest.raises(ValueError, match="gamma"):
             ops._norm_gamma("gamma", t, 100, cpu)
-    for s in ([], range(17), [0, -1], [0, 2 ** 31]):
+    for s in ([], range(17), [0, -1], [0, 2 ** 31], [-1]):
         with pytest.raises(ValueError, match="segments"):
             ops._segments(s)
     assert ops._segments(None) == (None, 1) and list(ops._segments([0, 3])[0]) == [0, 3]
