@@ -32,14 +32,16 @@ struct QuantMx4Args {
   uint8_t* __restrict__ q;
   uint8_t* __restrict__ scale;
   int64_t ldx, ldq;
-  int32_t rows, cols, cols_pad, row0;   // row0: the launch's first row, a multiple of 16
+  int32_t rows, cols, cols_pad, across, group0;   // units of a row; the launch's first group of rows
 };
 
 __global__ __launch_bounds__(kThreads) void quant_mx4_kernel(QuantMx4Args a) {
   __shared__ uint32_t scales[64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r0 = (int64_t)a.row0 + kUnitRows * (int64_t)blockIdx.x;
-  const int64_t k = (int64_t)kUnitCols * blockIdx.y + 8 * lane;
+  // Units in the order of memory: a row's one after another.
+  const int group = (int)(blockIdx.x / (uint32_t)a.across), slab = (int)blockIdx.x - group * a.across;
+  const int64_t r0 = kUnitRows * (int64_t)(a.group0 + group);
+  const int64_t k = (int64_t)kUnitCols * slab + 8 * lane;
   const int b = lane >> 2;                   // the lane's block of the unit
   u32x4 v[4];
 #pragma unroll
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(kThreads) void quant_mx4_kernel(QuantMx4Args a) {
   __syncthreads();
   if (wave == 0) {
     const int64_t blocks = ((int64_t)a.rows + kUnitRows - 1) / kUnitRows;
-    reinterpret_cast<uint32_t*>(a.scale)[64 * (blocks * blockIdx.y + r0 / kUnitRows) + lane] =
+    reinterpret_cast<uint32_t*>(a.scale)[64 * (blocks * slab + r0 / kUnitRows) + lane] =
         scales[lane];
   }
 }
@@ -70,15 +72,17 @@ struct DequantMx4Args {
   const uint8_t* __restrict__ scale;
   uint16_t* __restrict__ x;
   int64_t ldq, ldx;
-  int32_t rows, cols, row0;
+  int32_t rows, cols, across, group0;
 };
 
 __global__ __launch_bounds__(kThreads) void dequant_mx4_kernel(DequantMx4Args a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r0 = (int64_t)a.row0 + kUnitRows * (int64_t)blockIdx.x;
-  const int64_t k = (int64_t)kUnitCols * blockIdx.y + 8 * lane;
+  // Units in the order of memory: a row's one after another.
+  const int group = (int)(blockIdx.x / (uint32_t)a.across), slab = (int)blockIdx.x - group * a.across;
+  const int64_t r0 = kUnitRows * (int64_t)(a.group0 + group);
+  const int64_t k = (int64_t)kUnitCols * slab + 8 * lane;
   const int64_t blocks = ((int64_t)a.rows + kUnitRows - 1) / kUnitRows;
-  const uint8_t* scales = a.scale + 256 * (blocks * blockIdx.y + r0 / kUnitRows);
+  const uint8_t* scales = a.scale + 256 * (blocks * slab + r0 / kUnitRows);
   const int b = lane >> 2;
   if (k >= a.cols) return;
   uint32_t codes[4], bytes[4];
@@ -111,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void dequant_mx4_kernel(DequantMx4Args a)
   }
 }
 
-// A launch takes fewer than 2^32 threads and 65,536 units across.
+// A launch takes fewer than 2^32 threads.
 constexpr int64_t kMaxUnits = (int64_t)1 << 23;
 constexpr int32_t kMaxCols = 65535 * kUnitCols;
 
@@ -119,8 +123,14 @@ bool aligned(const void* p, uintptr_t to) {
   return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0;
 }
 
-// Rows a launch of `across` units a row of units takes.
-int64_t rows_at_once(int across) { return std::max<int64_t>(1, kMaxUnits / across) * kUnitRows; }
+// launch(first group of rows, workgroups) until all of them are through.
+template <class Launch>
+void for_all_groups(int32_t rows, int across, const Launch& launch) {
+  const int64_t groups = ((int64_t)rows + kUnitRows - 1) / kUnitRows;
+  const int64_t at_once = kMaxUnits / across;
+  for (int64_t g = 0; g < groups; g += at_once)
+    launch((int32_t)g, (unsigned)(std::min(groups - g, at_once) * across));
+}
 
 }  // namespace
 
@@ -141,13 +151,11 @@ extern "C" int h3hip_quant_rows_mx4(const void* x, int64_t ldx, int32_t rows, in
   H3_REQUIRE(aligned(x, 2) && aligned(q, 16) && aligned(scale, 4), H3HIP_EINVAL,
              "x must be 2-byte, q 16-byte and scale 4-byte aligned");
   const int across = (cols_pad + kUnitCols - 1) / kUnitCols;
-  for (int64_t r = 0; r < rows; r += rows_at_once(across)) {
-    const int64_t n = std::min<int64_t>(rows - r, rows_at_once(across));
-    const dim3 grid((unsigned)((n + kUnitRows - 1) / kUnitRows), (unsigned)across);
-    quant_mx4_kernel<<<grid, kThreads, 0, as_stream(stream)>>>(
+  for_all_groups(rows, across, [&](int32_t group0, unsigned grid) {
+    quant_mx4_kernel<<<dim3(grid), kThreads, 0, as_stream(stream)>>>(
         QuantMx4Args{static_cast<const uint16_t*>(x), static_cast<uint8_t*>(q),
-                     static_cast<uint8_t*>(scale), ldx, ldq, rows, cols, cols_pad, (int32_t)r});
-  }
+                     static_cast<uint8_t*>(scale), ldx, ldq, rows, cols, cols_pad, across, group0});
+  });
   return check_launch("quant_mx4_kernel");
 }
 
@@ -162,12 +170,10 @@ extern "C" int h3hip_dequant_rows_mx4(const void* q, int64_t ldq, const void* sc
   H3_REQUIRE(q && scale && x, H3HIP_EINVAL, "NULL tensor argument");
   H3_REQUIRE(aligned(x, 2) && aligned(q, 4), H3HIP_EINVAL, "x must be 2-byte, q 4-byte aligned");
   const int across = (cols + kUnitCols - 1) / kUnitCols;
-  for (int64_t r = 0; r < rows; r += rows_at_once(across)) {
-    const int64_t n = std::min<int64_t>(rows - r, rows_at_once(across));
-    const dim3 grid((unsigned)((n + kUnitRows - 1) / kUnitRows), (unsigned)across);
-    dequant_mx4_kernel<<<grid, kThreads, 0, as_stream(stream)>>>(
+  for_all_groups(rows, across, [&](int32_t group0, unsigned grid) {
+    dequant_mx4_kernel<<<dim3(grid), kThreads, 0, as_stream(stream)>>>(
         DequantMx4Args{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale),
-                       static_cast<uint16_t*>(x), ldq, ldx, rows, cols, (int32_t)r});
-  }
+                       static_cast<uint16_t*>(x), ldq, ldx, rows, cols, across, group0});
+  });
   return check_launch("dequant_mx4_kernel");
 }
