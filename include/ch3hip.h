@@ -424,7 +424,7 @@ int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features, int32_t he
 /* A norm over the hidden width with its modulation: of a row x of segment s
  *   x rsqrt(mean x^2 + eps) gamma (1 + scale[s]) + shift[s]
  * All tables device bf16 and optional: gamma [hidden] (NULL: 1), scale and shift
- * [segments, hidden] with row strides in elements (NULL: 0). */
+ * [segments, hidden] with row strides in elements (NULL: 0; stride 0: one row for all). */
 typedef struct {
   const void* gamma;
   const void* scale;
@@ -454,8 +454,8 @@ int h3hip_norm_modulate(const void* x, int64_t ldx, int32_t rows, int32_t hidden
  * rounded to bf16 only as r). fp32 up to those roundings.
  *   x, y, r, h: device bf16 [rows, hidden], row strides in elements; rows may begin anywhere.
  *      r or h may be x or y (the same address and stride), and no other overlap is allowed.
- *   gate: device bf16 [segments, hidden], row stride ld_gate (NULL: 1); post_gamma: device
- *      bf16 [hidden] or NULL. next: a host struct or NULL (h unused).
+ *   gate: device bf16 [segments, hidden], row stride ld_gate (0: one row for all; NULL: 1);
+ *      post_gamma: device bf16 [hidden] or NULL. next: a host struct or NULL (h unused).
  * Everything else as for h3hip_norm_modulate. */
 int h3hip_gated_residual(const void* x, int64_t ldx, const void* y, int64_t ldy, int32_t rows,
                          int32_t hidden, const void* gate, int64_t ld_gate,

@@ -283,6 +283,17 @@ int launch(const NormArgs& a, hipStream_t st) {
 
 bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 
+// A table's row stride; 0: every segment has the one row.
+bool covers(int64_t ld, int32_t hidden) { return ld >= hidden || ld == 0; }
+
+// Rows that an output overwrites have to be the same rows.
+int check_in_place(const void* out, int64_t ldo, const void* in, int64_t ldi, int32_t rows) {
+  H3_REQUIRE(out != in || ldo == ldi || rows == 1, H3HIP_EINVAL,
+             "an output in place of an input needs its stride (%lld, not %lld)", (long long)ldi,
+             (long long)ldo);
+  return H3HIP_OK;
+}
+
 // Sizes and segments, which both entry points share.
 int check_sizes(int32_t rows, int32_t hidden, const int32_t* starts, int32_t segments) {
   H3_REQUIRE(rows >= 0 && hidden > 0, H3HIP_EINVAL, "bad shape: rows %d hidden %d", rows, hidden);
@@ -306,9 +317,9 @@ int check_sizes(int32_t rows, int32_t hidden, const int32_t* starts, int32_t seg
 int check_norm(const h3hip_norm* norm, int32_t hidden, int32_t segments) {
   H3_REQUIRE(aligned2(norm->gamma) && aligned2(norm->scale) && aligned2(norm->shift), H3HIP_EINVAL,
              "tensors must be 2-byte aligned");
-  H3_REQUIRE(segments == 1 || ((!norm->scale || norm->ld_scale >= hidden) &&
-                               (!norm->shift || norm->ld_shift >= hidden)),
-             H3HIP_EINVAL, "ld_scale %lld and ld_shift %lld must cover a row",
+  H3_REQUIRE(segments == 1 || ((!norm->scale || covers(norm->ld_scale, hidden)) &&
+                               (!norm->shift || covers(norm->ld_shift, hidden))),
+             H3HIP_EINVAL, "ld_scale %lld and ld_shift %lld must cover a row or be 0",
              (long long)norm->ld_scale, (long long)norm->ld_shift);
   return H3HIP_OK;
 }
@@ -349,6 +360,8 @@ extern "C" int h3hip_norm_modulate(const void* x, int64_t ldx, int32_t rows, int
   if (rows == 0) return H3HIP_OK;
   H3_REQUIRE(x && h, H3HIP_EINVAL, "NULL tensor argument");
   H3_REQUIRE(aligned2(x) && aligned2(h), H3HIP_EINVAL, "tensors must be 2-byte aligned");
+  rc = check_in_place(h, ldh, x, ldx, rows);
+  if (rc != H3HIP_OK) return rc;
   NormArgs a{};
   a.x = static_cast<const uint16_t*>(x);
   a.h = static_cast<uint16_t*>(h);
@@ -372,7 +385,7 @@ extern "C" int h3hip_gated_residual(const void* x, int64_t ldx, const void* y, i
     if (rc != H3HIP_OK) return rc;
   }
   H3_REQUIRE(ldx >= hidden && ldy >= hidden && ldr >= hidden && (!next || ldh >= hidden) &&
-                 (!gate || segments == 1 || ld_gate >= hidden),
+                 (!gate || segments == 1 || covers(ld_gate, hidden)),
              H3HIP_EINVAL, "ldx %lld, ldy %lld, ldr %lld, ldh %lld and ld_gate %lld must cover a row",
              (long long)ldx, (long long)ldy, (long long)ldr, (long long)ldh, (long long)ld_gate);
   if (rows == 0) return H3HIP_OK;
@@ -380,6 +393,12 @@ extern "C" int h3hip_gated_residual(const void* x, int64_t ldx, const void* y, i
   H3_REQUIRE(aligned2(x) && aligned2(y) && aligned2(r) && aligned2(h) && aligned2(gate) &&
                  aligned2(post_gamma),
              H3HIP_EINVAL, "tensors must be 2-byte aligned");
+  H3_REQUIRE(!next || r != h, H3HIP_EINVAL, "r and h must be two tensors");
+  rc = check_in_place(r, ldr, x, ldx, rows);
+  if (rc == H3HIP_OK) rc = check_in_place(r, ldr, y, ldy, rows);
+  if (rc == H3HIP_OK && next) rc = check_in_place(h, ldh, x, ldx, rows);
+  if (rc == H3HIP_OK && next) rc = check_in_place(h, ldh, y, ldy, rows);
+  if (rc != H3HIP_OK) return rc;
   NormArgs a{};
   a.x = static_cast<const uint16_t*>(x);
   a.y = static_cast<const uint16_t*>(y);

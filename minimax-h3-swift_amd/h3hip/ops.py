@@ -458,7 +458,8 @@ class Mx4Rows(NamedTuple):
     the low half (row stride free). scale: [slabs, ceil(S/16), 64, 4] uint8, the blocks' biased
     exponents in the order in which the kernels read them: row r's and block b's at
     [b // 16, r // 16, 16 * (b % 4) + r % 16, b // 4 % 4]. cols: values of a row.
-    quant_rows_mx4() makes them of bf16 rows, pack() of what a checkpoint holds."""
+    quant_rows_mx4() makes them of bf16 rows, pack() of what a checkpoint holds, rows() of some of
+    the rows (the scales belong to all rows from the first on: values alone are not sliced)."""
     values: torch.Tensor
     scale: torch.Tensor
     cols: int
@@ -493,6 +494,16 @@ class Mx4Rows(NamedTuple):
         # [group, row, slab, byte, quarter] -> [slab, group, quarter, row, byte]
         scale = rows.view(groups, 16, slabs, 4, 4).permute(2, 0, 4, 1, 3)
         return cls(values, scale.reshape(slabs, groups, 64, 4).contiguous(), cols)
+
+    def rows(self, first: int, count: int) -> "Mx4Rows":
+        """Some of the rows (a weight's channels of one rank, a part of the tokens), from a
+        multiple of 16 on: the values in place, their scales copied."""
+        S = self.values.shape[0]
+        if first % 16 or not 0 <= first <= first + count <= S:
+            raise ValueError(f"rows must begin at a multiple of 16 and lie in 0..{S}, got {first} + "
+                             f"{count}")
+        scale = self.scale[:, first // 16:(first + count + 15) // 16].contiguous()
+        return Mx4Rows(self.values[first:first + count], scale, self.cols)
 
     def exponents(self) -> torch.Tensor:
         """The biased exponents row-major, [S, ceil(cols/32)] uint8: what pack() takes."""
@@ -771,7 +782,7 @@ def _segments(starts):
         raise ValueError(f"segments must be 1 to 16 first rows, got {n}")
     if min(starts) < 0 or max(starts) > _INT32_MAX:
         raise ValueError(f"segments must be rows from 0 to below 2^31, got {list(starts)}")
-    return _Starts[n](*starts), n
+    return _Starts[n](*map(int, starts)), n
 
 
 def norm_modulate(x: torch.Tensor, gamma: torch.Tensor | None = None,

@@ -309,3 +309,18 @@ def test_captured_replayed_and_on_two_streams(h3):
         want = [bits16(t) for t in run(a, b)]
         for o in outs[i]:
             assert all((bits16(t) == w).all() for t, w in zip(o, want))
+
+
+def test_one_modulation_for_every_segment(h3):
+    """Tables expanded over the segments: a row stride of 0."""
+    from h3hip import ops
+    x, y, tab = _inputs(60, 1000, 3)
+    wide = {k: tab[k].expand(4, 1000) for k in ("scale", "shift", "gate")}
+    norm = dict(gamma=tab["gamma"], scale=wide["scale"], shift=wide["shift"])
+    a = ops.gated_residual(x, y, wide["gate"], segments=[0, 5, 9, 30], next_norm=norm)
+    b = ops.gated_residual(x, y, tab["gate"], next_norm=dict(gamma=tab["gamma"], scale=tab["scale"],
+                                                             shift=tab["shift"]))
+    for t, u in zip(a, b):
+        assert (bits16(t) == bits16(u)).all()
+    a = ops.norm_modulate(x, **norm, segments=[0, 5, 9, 30])
+    assert (bits16(a) == bits16(ops.norm_modulate(x, tab["gamma"], tab["scale"], tab["shift"]))).all()

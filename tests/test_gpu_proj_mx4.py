@@ -278,3 +278,14 @@ def test_decoding_of_the_tests_own(h3):
     from h3hip import ops
     x = mx4_operand(37, 777, 1, -30, 60)
     assert torch.equal(decode64(x), ops.dequant_rows_mx4(x).double())
+
+
+@pytest.mark.parametrize("first,S,N", [(16, 3, 100), (0, 300, 517), (32, 700, 640)])
+def test_some_rows_of_a_weight(h3, first, S, N):
+    """rows() of a weight: those channels' bits."""
+    from h3hip import ops
+    x, w = mx4_operand(S, 512, S, -5, 10), mx4_operand(N + 41, 512, N, -5, 10)
+    note(f"proj_mx4 channels {first}.. of {N + 41}, S={S}")
+    every = bits16(ops.proj_mx4(x, w))
+    some = bits16(ops.proj_mx4(x, w.rows(first, N)))
+    assert (some == every[:, first:first + N]).all()

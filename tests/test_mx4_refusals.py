@@ -231,3 +231,21 @@ def test_sizes_past_32_bits(h3, S, K):
         ops.dequant_rows_mx4(rows)
     with pytest.raises(ValueError, match="2\\^31"):
         ops.proj_mx4(rows, rows)
+
+
+def test_some_of_the_rows(h3):
+    g = torch.Generator()
+    g.manual_seed(1)
+    from h3hip import ops
+    codes = torch.randint(0, 256, (70, 20), generator=g, dtype=torch.uint8)
+    e = torch.randint(0, 256, (70, 2), generator=g, dtype=torch.uint8)
+    rows = ops.Mx4Rows.pack(codes, e, 39)
+    for first, count in ((0, 70), (16, 16), (32, 5), (48, 22), (64, 0)):
+        part, want = rows.rows(first, count), ops.Mx4Rows.pack(codes[first:first + count],
+                                                               e[first:first + count], 39)
+        assert torch.equal(part.values, want.values) and part.cols == 39
+        assert torch.equal(part.exponents(), want.exponents())
+        assert part.scale.shape == want.scale.shape
+    for first, count in ((8, 4), (64, 7), (-16, 4), (0, -1)):
+        with pytest.raises(ValueError, match="multiple of 16"):
+            rows.rows(first, count)

@@ -8,6 +8,7 @@ import torch
 
 BUF = ctypes.c_void_p(4096)       # an aligned address no refused call reads
 ODD = ctypes.c_void_p(4097)
+AWAY = ctypes.c_void_p(1 << 20)
 NONE = object()
 
 
@@ -44,7 +45,11 @@ SHARED = [(dict(rows=-1), "shape"), (dict(hidden=0), "shape"), (dict(segments=0)
           (dict(norm=("ld_scale", 99)), "cover"), (dict(norm=("ld_shift", 99)), "cover")]
 AFTER = [(dict(ldy=99), "cover"), (dict(ldr=99), "cover"), (dict(ld_gate=99), "cover"),
          (dict(y=None), "NULL"), (dict(r=None), "NULL"), (dict(y=ODD), "aligned"),
-         (dict(r=ODD), "aligned"), (dict(gate=ODD), "aligned"), (dict(post=ODD), "aligned")]
+         (dict(r=ODD), "aligned"), (dict(gate=ODD), "aligned"), (dict(post=ODD), "aligned"),
+         # r, h, x and y are one address in these calls, which in place they have to be with one
+         # stride; r and h never.
+         (dict(), "two tensors"), (dict(h=AWAY, ldr=104), "stride"), (dict(r=AWAY, ldh=104), "stride"),
+         (dict(h=AWAY, ldy=104), "stride"), (dict(r=AWAY, ldy=104), "stride")]
 
 
 def _args(bad):
@@ -54,7 +59,7 @@ def _args(bad):
     return bad
 
 
-@pytest.mark.parametrize("bad,word", SHARED + [(dict(norm=NONE), "NULL")])
+@pytest.mark.parametrize("bad,word", SHARED + [(dict(norm=NONE), "NULL"), (dict(ldh=104), "stride")])
 def test_norm_modulate(h3, bad, word):
     from h3hip import _lib
     assert _before(h3, **_args(bad)) == _lib.EINVAL and word in h3.last_error()
@@ -106,6 +111,8 @@ def test_wrapper_checks_of_tables(h3):
     for t in (good, good[0, :99], good[0].float(), torch.zeros(200, dtype=torch.bfloat16)[::2]):
         with pytest.raises(ValueError, match="gamma"):
             ops._norm_gamma("gamma", t, 100, cpu)
+    import numpy as np
+    assert list(ops._segments(np.array([0, 3]))[0]) == list(ops._segments(torch.tensor([0, 3]))[0])
     for s in ([], range(17), [0, -1], [0, 2 ** 31], [-1]):
         with pytest.raises(ValueError, match="segments"):
             ops._segments(s)
