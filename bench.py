@@ -603,7 +603,8 @@ def attention_layer_extra(args, env):
     (torch.mm); and hipBLASLt's GEMMs with the prologue kernel between them
     (V then read in place from the token-major qkv). The out-projection alone
     is timed both ways beside them. Then the first path in turn with the same layer on
-    int8 projections (weights rounded before, activations in the timed call)."""
+    int8 and on microscaled 4-bit projections (weights rounded before, activations in the
+    timed call)."""
     import numpy as np
     import torch
     from h3hip import ops
@@ -687,6 +688,22 @@ def attention_layer_extra(args, env):
     res["int8_projections"] = {"timing": "medians of interleaved calls",
                                "int8_ms": round(med["int8"], 4), "bf16_ms": round(med["bf16"], 4),
                                "rel_rms_vs_bf16": round(rel, 5)}
+
+    w4, w4_out = ops.quant_rows_mx4(w), ops.quant_rows_mx4(w_out)
+    y4 = torch.empty_like(y)
+
+    def mx4_path():
+        ops.qkv_proj_mx4(x, w4, env["gq"], env["gk"], table, heads=H, eps=eps, seq_pad=S_pad,
+                         out=(qh, kh, vh))
+        ops.bsattn_fwd_strided(plan, qh, kh, vh, scale, out=att_view)
+        ops.proj_mx4(att, w4_out, out=y4)
+
+    med = interleaved_medians({"bf16": all_h3hip_path, "mx4": mx4_path},
+                              reps=max(12, args.steps))
+    rel = float((y4.double() - y.double()).norm() / y.double().norm())
+    res["mx4_projections"] = {"timing": "medians of interleaved calls",
+                              "mx4_ms": round(med["mx4"], 4), "bf16_ms": round(med["bf16"], 4),
+                              "rel_rms_vs_bf16": round(rel, 5)}
     return res
 
 
