@@ -10,8 +10,8 @@
 // from the rounded one.
 //
 // Bound by HBM: before 4 bytes an element, after with a next norm 8 (31,885 x 5,120: 137 us, 4.8
-// TB/s, and 265 us, 4.9; a copy of 1 GiB 5.1), of few rows by the launch (125 x 5,120: 4.2 us). So a row is read once and
-// stays in registers through its sums, and the tables, which as rows are as long as x's, are held
+// TB/s, and 265 us, 4.9; a copy of 1 GiB 5.1), of few rows by the launch (125 x 5,120: 4.2 us). So a
+// row is read once and stays in registers through its sums, and the tables, which as rows are as long as x's, are held
 // in registers too, by workers that take a range of consecutive rows each and reload the
 // tables only where a segment begins. The next row's loads are in flight while one is summed (of
 // widths up to 8,192).

@@ -14,7 +14,10 @@
 // consecutive bytes, and the unit of work here: a workgroup reads them 16 bytes a lane, 4
 // lanes a block, and collects their scales in LDS.
 //
-// Bound by HBM: 2 bytes read and 17/32 written an element.
+// Bound by HBM: 2 bytes read and 17/32 written an element, and the other way round: 31,885 x 5,120,
+// x in no cache, 74 us to 4 bits (5.6 TB/s) and 75 back. Workgroups take units in the order of memory;
+// down the columns first they took 82.6 and 86, two units a workgroup 78. 637 x 1,001 is a launch and
+// two latencies, 4.0 us.
 #include <algorithm>
 #include <climits>
 
