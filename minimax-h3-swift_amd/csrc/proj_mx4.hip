@@ -143,6 +143,9 @@ int linear(const ProjArgs& o, const void* x, int64_t ldx, const void* w, int64_t
   H3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
              H3HIP_EINVAL, "a workspace of %lld bytes, 16-byte aligned, is needed (%lld given)",
              (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  // Before the rows are rounded: what no tile shape takes, the largest does not.
+  H3_REQUIRE(proj_mx4_fits(o.seq_len, n_total, kProjMx4Shapes[0]), H3HIP_EINVAL,
+             "too many rows or channels for one launch (%d x %d)", o.seq_len, n_total);
   if (few_mx4_takes(o.seq_len, in)) {
     float* sums = out ? nullptr : static_cast<float*>(workspace);
     const int rc = launch_few_mx4(

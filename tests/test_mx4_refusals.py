@@ -249,3 +249,16 @@ def test_some_of_the_rows(h3):
     for first, count in ((8, 4), (64, 7), (-16, 4), (0, -1)):
         with pytest.raises(ValueError, match="multiple of 16"):
             rows.rows(first, count)
+
+
+@pytest.mark.parametrize("rows,k", [(1, 512), (2, 512), (1, 500), (3, 512), (16_776_961, 512)])
+def test_too_many_rows_or_channels(h3, rows, k):
+    """No launch holds them: refused before the rows are rounded, by the form for few rows too."""
+    from h3hip import _lib
+    n = 64 if rows > 3 else 16_776_961
+    big = dict(rows=rows, k=k, ldx=512, n=n, ldy=1 << 26, size=1 << 50)
+    assert _linear(h3, **big) == _lib.EINVAL and "too many" in h3.last_error()
+    heads = 1 if rows > 3 else 43_691          # 3 * 43,691 * 128 channels
+    pad = (rows + 127) // 128 * 128
+    assert (_qkv_linear(h3, S=rows, pad=pad, k=k, ldx=512, H=heads, size=1 << 50) == _lib.EINVAL
+            and "too many" in h3.last_error())
