@@ -36,7 +36,10 @@ constexpr int kCus = 256;
 // 11 waves did not fit a CU (31,885 x 5,376, after with a next norm, 373 us; 290).
 constexpr int kWavesCu = 24;
 
-struct NormArgs {
+// What a launch needs where one segment holds every row: 120 bytes, because the host takes 0.9 us
+// longer for a launch of 128 bytes of arguments and more (the kernel's use of the launch's
+// dimensions counts 256 of them, so they are made of hidden here).
+struct NormRows {
   const uint16_t* x;                       // r or h may be x or y
   const uint16_t* y;
   uint16_t* r;
@@ -46,11 +49,29 @@ struct NormArgs {
   const uint16_t* __restrict__ gamma;
   const uint16_t* __restrict__ scale;
   const uint16_t* __restrict__ shift;
-  int64_t ldx, ldy, ldr, ldh, ld_gate, ld_scale, ld_shift;
+  int64_t ldx, ldy, ldr, ldh;
   float alpha, eps;
-  int32_t rows, hidden, segments;
+  int32_t rows;
+  uint16_t hidden, workers_cu;             // workgroups a CU
+};
+template <bool kMany>
+struct NormArgs : NormRows {};
+template <>
+struct NormArgs<true> : NormRows {
+  int64_t ld_gate, ld_scale, ld_shift;
+  int32_t segments;
   int32_t starts[kMaxSegments];
 };
+
+// Waves of a row of `hidden` elements, and its workgroups (fewer where there are fewer rows).
+template <int kChunks>
+__host__ __device__ constexpr int waves_of(int hidden) {
+  return (hidden + 64 * kLaneElems * kChunks - 1) / (64 * kLaneElems * kChunks);
+}
+__host__ __device__ constexpr int workers_of(int rows, int workers_cu) {
+  const int most = kCus * workers_cu;
+  return rows < most ? rows : most;
+}
 
 // 8 elements from k on, zeros past n. Rows may begin anywhere.
 __device__ __forceinline__ u32x4 load8(const uint16_t* row, int k, int n) {
@@ -92,6 +113,13 @@ __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
   return v;
 }
 
+// A uniform row number that the compiler makes no running addresses of: they took 8 registers a
+// thread more, past the 80 that there are.
+__device__ __forceinline__ int opaque(int row) {
+  asm("" : "+s"(row));
+  return row;
+}
+
 template <int kCtrl>
 __device__ __forceinline__ float dpp(float v) {
   return __uint_as_float(
@@ -111,20 +139,23 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // kChunks chunks of a row a thread. kAfter: there is y; kPost: it is normalised; kNext: h is
-// written (without kAfter always).
-template <int kChunks, bool kAfter, bool kPost, bool kNext>
+// written (without kAfter always); kMany: rows of more than one segment.
+template <int kChunks, bool kAfter, bool kPost, bool kNext, bool kMany>
 __global__ __launch_bounds__(kMaxThreads) __attribute__((amdgpu_waves_per_eu(kChunks == 1 ? 6 : 4)))
-void norm_residual_kernel(NormArgs a) {
+void norm_residual_kernel(NormArgs<kMany> a) {
   constexpr int kSums = (kPost ? 1 : 0) + (kNext ? 1 : 0);
   constexpr int kMaxWaves = kMaxThreads / 64;
   __shared__ __attribute__((aligned(16))) float part[2][kSums > 0 ? kSums : 1][kMaxWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int waves = (int)blockDim.x >> 6;
-  const int first = (int)((int64_t)blockIdx.x * a.rows / gridDim.x);
-  const int last = (int)(((int64_t)blockIdx.x + 1) * a.rows / gridDim.x);
-  const int k0 = kLaneElems * (int)threadIdx.x, n = a.hidden;
-  const int stride = kLaneElems * (int)blockDim.x;
+  const int n = a.hidden, waves = waves_of<kChunks>(n);
+  // Rows first to last - 1: as many for every worker, one more for the first of them.
+  const uint32_t workers = (uint32_t)workers_of(a.rows, a.workers_cu), rows = (uint32_t)a.rows;
+  const uint32_t share = rows / workers, more = rows - share * workers;
+  const int first = (int)(blockIdx.x * share + min(blockIdx.x, more));
+  const int last = first + (int)(share + (blockIdx.x < more ? 1 : 0));
+  const int k0 = kLaneElems * (int)threadIdx.x;
+  const int stride = 64 * kLaneElems * waves;
   const float inv_n = 1.0f / (float)n;
   // Slots of waves that do not exist add as zeros.
   if (waves > 1 && (int)threadIdx.x < 2 * (kSums > 0 ? kSums : 1) * kMaxWaves)
@@ -146,7 +177,8 @@ void norm_residual_kernel(NormArgs a) {
   };
 
   u32x4 vx[kChunks], vy[kChunks];
-  auto load_row = [&](int row, u32x4 (&tx)[kChunks], u32x4 (&ty)[kChunks]) __attribute__((always_inline)) {
+  auto load_row = [&](int at, u32x4 (&tx)[kChunks], u32x4 (&ty)[kChunks]) __attribute__((always_inline)) {
+    const int row = opaque(at);
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
       const int k = k0 + c * stride;
@@ -161,6 +193,9 @@ void norm_residual_kernel(NormArgs a) {
   // row's segment.
   float fg[kAfter ? kChunks : 1][8], fa[kNext ? kChunks : 1][8], fb[kNext ? kChunks : 1][8];
   auto load_tables = [&](int s) __attribute__((always_inline)) {
+    int64_t gate_at = 0, scale_at = 0, shift_at = 0;
+    if constexpr (kMany)
+      gate_at = s * a.ld_gate, scale_at = s * a.ld_scale, shift_at = s * a.ld_shift;
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
       const int k = k0 + c * stride;
@@ -168,7 +203,7 @@ void norm_residual_kernel(NormArgs a) {
         float t[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) fg[c][i] = 1.0f;
-        if (a.gate) unpack(load8(a.gate + s * a.ld_gate, k, n), fg[c]);
+        if (a.gate) unpack(load8(a.gate + gate_at, k, n), fg[c]);
         if constexpr (kPost) {
           unpack(load8(a.post, k, n), t);
 #pragma unroll
@@ -181,24 +216,27 @@ void norm_residual_kernel(NormArgs a) {
         for (int i = 0; i < 8; i++) fa[c][i] = 1.0f, fb[c][i] = 0.0f;
         if (a.gamma) unpack(load8(a.gamma, k, n), fa[c]);
         if (a.scale) {
-          unpack(load8(a.scale + s * a.ld_scale, k, n), t);
+          unpack(load8(a.scale + scale_at, k, n), t);
 #pragma unroll
           for (int i = 0; i < 8; i++) fa[c][i] *= 1.0f + t[i];
         }
-        if (a.shift) unpack(load8(a.shift + s * a.ld_shift, k, n), fb[c]);
+        if (a.shift) unpack(load8(a.shift + shift_at, k, n), fb[c]);
       }
     }
   };
   int until = first;                       // the row at which the tables change
+  if constexpr (!kMany) load_tables(0);
   for (int row = first; row < last; row++) {
-    if (row >= until) {
-      int s = 0;
-      until = INT_MAX;
-      for (int i = 1; i < a.segments; i++) {
-        if (a.starts[i] <= row) s = i;
-        else until = min(until, a.starts[i]);
+    if constexpr (kMany) {
+      if (row >= until) {
+        int s = 0;
+        until = INT_MAX;
+        for (int i = 1; i < a.segments; i++) {
+          if (a.starts[i] <= row) s = i;
+          else until = min(until, a.starts[i]);
+        }
+        load_tables(s);
       }
-      load_tables(s);
     }
     u32x4 nx[kChunks], ny[kChunks];
     if (!kAhead)
@@ -229,7 +267,7 @@ void norm_residual_kernel(NormArgs a) {
         unpack(vy[c], t);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[c][i] = a.alpha * v[c][i] + fg[c][i] * (t[i] * rs);
-        store8<kNext>(a.r + row * a.ldr, k0 + c * stride, n, pack(v[c]));
+        store8<kNext>(a.r + opaque(row) * a.ldr, k0 + c * stride, n, pack(v[c]));
       }
     }
     if constexpr (kNext) {
@@ -244,7 +282,7 @@ void norm_residual_kernel(NormArgs a) {
         float t[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) t[i] = v[c][i] * rs * fa[c][i] + fb[c][i];
-        store8<false>(a.h + row * a.ldh, k0 + c * stride, n, pack(t));
+        store8<false>(a.h + opaque(row) * a.ldh, k0 + c * stride, n, pack(t));
       }
     }
     if constexpr (kAhead) {
@@ -257,27 +295,51 @@ void norm_residual_kernel(NormArgs a) {
   }
 }
 
-template <int kChunks>
-void launch(const NormArgs& a, hipStream_t st) {
-  const int waves = (a.hidden + 64 * kLaneElems * kChunks - 1) / (64 * kLaneElems * kChunks);
-  const dim3 block(64 * waves);
-  const dim3 grid((unsigned)std::min(a.rows, kCus * std::max(1, kWavesCu / waves)));
+template <int kChunks, bool kMany>
+void launch_chunks(const NormArgs<kMany>& a, hipStream_t st) {
+  const dim3 block(64 * waves_of<kChunks>(a.hidden));
+  const dim3 grid((unsigned)workers_of(a.rows, a.workers_cu));
   const bool next = a.h != nullptr;
   if (a.y == nullptr)
-    norm_residual_kernel<kChunks, false, false, true><<<grid, block, 0, st>>>(a);
+    norm_residual_kernel<kChunks, false, false, true, kMany><<<grid, block, 0, st>>>(a);
   else if (a.post && next)
-    norm_residual_kernel<kChunks, true, true, true><<<grid, block, 0, st>>>(a);
+    norm_residual_kernel<kChunks, true, true, true, kMany><<<grid, block, 0, st>>>(a);
   else if (a.post)
-    norm_residual_kernel<kChunks, true, true, false><<<grid, block, 0, st>>>(a);
+    norm_residual_kernel<kChunks, true, true, false, kMany><<<grid, block, 0, st>>>(a);
   else if (next)
-    norm_residual_kernel<kChunks, true, false, true><<<grid, block, 0, st>>>(a);
+    norm_residual_kernel<kChunks, true, false, true, kMany><<<grid, block, 0, st>>>(a);
   else
-    norm_residual_kernel<kChunks, true, false, false><<<grid, block, 0, st>>>(a);
+    norm_residual_kernel<kChunks, true, false, false, kMany><<<grid, block, 0, st>>>(a);
 }
 
-int launch(const NormArgs& a, hipStream_t st) {
-  if (a.hidden <= kMaxThreads * kLaneElems) launch<1>(a, st);
-  else launch<2>(a, st);
+template <bool kMany>
+void launch(const NormArgs<kMany>& a, hipStream_t st) {
+  if (a.hidden <= kMaxThreads * kLaneElems) launch_chunks<1>(a, st);
+  else launch_chunks<2>(a, st);
+}
+
+// Fills in the sizes and launches; a's tables are the first segment's.
+int launch(NormArgs<true>& a, int32_t rows, int32_t hidden, float eps, const int32_t* starts,
+           int32_t segments, void* stream) {
+  const int waves = hidden <= kMaxThreads * kLaneElems ? waves_of<1>(hidden) : waves_of<2>(hidden);
+  a.rows = rows;
+  a.hidden = (uint16_t)hidden;
+  a.workers_cu = (uint16_t)std::max(1, kWavesCu / waves);
+  a.eps = eps;
+  a.segments = segments;
+  for (int i = 1; i < segments; i++) a.starts[i] = starts[i];
+  // The last segment that begins at row 0, and whether another row's begins after it.
+  int s = 0;
+  while (s + 1 < segments && starts[s + 1] == 0) s++;
+  if (s + 1 < segments && starts[s + 1] < rows) {
+    launch<true>(a, as_stream(stream));
+  } else {
+    NormArgs<false> one{a};
+    if (one.gate) one.gate += s * a.ld_gate;
+    if (one.scale) one.scale += s * a.ld_scale;
+    if (one.shift) one.shift += s * a.ld_shift;
+    launch<false>(one, as_stream(stream));
+  }
   return check_launch("norm_residual_kernel");
 }
 
@@ -324,21 +386,12 @@ int check_norm(const h3hip_norm* norm, int32_t hidden, int32_t segments) {
   return H3HIP_OK;
 }
 
-void set_norm(NormArgs& a, const h3hip_norm* norm) {
+void set_norm(NormArgs<true>& a, const h3hip_norm* norm) {
   a.gamma = static_cast<const uint16_t*>(norm->gamma);
   a.scale = static_cast<const uint16_t*>(norm->scale);
   a.shift = static_cast<const uint16_t*>(norm->shift);
   a.ld_scale = norm->ld_scale;
   a.ld_shift = norm->ld_shift;
-}
-
-void set_sizes(NormArgs& a, int32_t rows, int32_t hidden, const int32_t* starts, int32_t segments,
-               float eps) {
-  a.rows = rows;
-  a.hidden = hidden;
-  a.segments = segments;
-  a.eps = eps;
-  for (int i = 1; i < segments; i++) a.starts[i] = starts[i];
 }
 
 }  // namespace
@@ -362,14 +415,13 @@ extern "C" int h3hip_norm_modulate(const void* x, int64_t ldx, int32_t rows, int
   H3_REQUIRE(aligned2(x) && aligned2(h), H3HIP_EINVAL, "tensors must be 2-byte aligned");
   rc = check_in_place(h, ldh, x, ldx, rows);
   if (rc != H3HIP_OK) return rc;
-  NormArgs a{};
+  NormArgs<true> a{};
   a.x = static_cast<const uint16_t*>(x);
   a.h = static_cast<uint16_t*>(h);
   a.ldx = ldx;
   a.ldh = ldh;
   set_norm(a, norm);
-  set_sizes(a, rows, hidden, starts, segments, eps);
-  return launch(a, as_stream(stream));
+  return launch(a, rows, hidden, eps, starts, segments, stream);
 }
 
 extern "C" int h3hip_gated_residual(const void* x, int64_t ldx, const void* y, int64_t ldy,
@@ -399,7 +451,7 @@ extern "C" int h3hip_gated_residual(const void* x, int64_t ldx, const void* y, i
   if (rc == H3HIP_OK && next) rc = check_in_place(h, ldh, x, ldx, rows);
   if (rc == H3HIP_OK && next) rc = check_in_place(h, ldh, y, ldy, rows);
   if (rc != H3HIP_OK) return rc;
-  NormArgs a{};
+  NormArgs<true> a{};
   a.x = static_cast<const uint16_t*>(x);
   a.y = static_cast<const uint16_t*>(y);
   a.r = static_cast<uint16_t*>(r);
@@ -413,6 +465,5 @@ extern "C" int h3hip_gated_residual(const void* x, int64_t ldx, const void* y, i
   a.ld_gate = ld_gate;
   a.alpha = residual_scale;
   if (next) set_norm(a, next);
-  set_sizes(a, rows, hidden, starts, segments, eps);
-  return launch(a, as_stream(stream));
+  return launch(a, rows, hidden, eps, starts, segments, stream);
 }

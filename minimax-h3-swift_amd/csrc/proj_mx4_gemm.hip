@@ -8,22 +8,23 @@ namespace h3hip {
 namespace {
 
 template <int kNA, int kMB, bool kPair>
-int launch(ProjMx4Args a, int32_t rounding, bool plain, bool out, hipStream_t st) {
-  const dim3 grid = order_grid<kNA, kMB>(a);
+int launch(const ProjMx4Args& a, int32_t rounding, bool plain, bool out, hipStream_t st) {
+  dim3 grid;
+  const ProjMx4Packed p = pack_args<kNA, kMB>(a, out, grid);
   constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32;
   if (out) {
-    proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 8, true, true><<<grid, kThreads, 0, st>>>(a);
+    proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 8, true, true><<<grid, kThreads, 0, st>>>(p);
   } else if constexpr (kNA >= 4) {
     if (plain)
-      proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 8, true, false><<<grid, kThreads, 0, st>>>(a);
+      proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 8, true, false><<<grid, kThreads, 0, st>>>(p);
     else if (rounding == kRef && a.out.rot == 128)
-      proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 8, false, false><<<grid, kThreads, 0, st>>>(a);
+      proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 8, false, false><<<grid, kThreads, 0, st>>>(p);
     else if (rounding == kRef)
-      proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+      proj_mx4_gemm_kernel<kNA, kMB, kPair, kRef, 6, false, false><<<grid, kThreads, 0, st>>>(p);
     else if (a.out.rot == 128)
-      proj_mx4_gemm_kernel<kNA, kMB, kPair, kF32, 8, false, false><<<grid, kThreads, 0, st>>>(a);
+      proj_mx4_gemm_kernel<kNA, kMB, kPair, kF32, 8, false, false><<<grid, kThreads, 0, st>>>(p);
     else
-      proj_mx4_gemm_kernel<kNA, kMB, kPair, kF32, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+      proj_mx4_gemm_kernel<kNA, kMB, kPair, kF32, 6, false, false><<<grid, kThreads, 0, st>>>(p);
   }
   return check_launch("proj_mx4_gemm_kernel");
 }

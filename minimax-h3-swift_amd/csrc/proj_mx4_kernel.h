@@ -103,8 +103,46 @@ __device__ __forceinline__ f32x4 block_sums(const f32x32 (&c)[kAccs<kNA, kMB>], 
   return y;
 }
 
+// A ProjMx4Args as the kernel takes it: a launch of 128 bytes of arguments and more takes the host
+// 0.9 us longer.
+struct ProjMx4Packed {
+  const uint8_t* __restrict__ x;
+  const uint8_t* __restrict__ w;
+  const uint8_t* __restrict__ x_scale;
+  const uint8_t* __restrict__ w_scale;
+  uint16_t* __restrict__ q_out;
+  uint16_t* __restrict__ k_out;
+  union {
+    uint16_t* v_out;
+    int64_t ldo;                           // of token rows
+  };
+  const uint16_t* __restrict__ q_gamma;
+  const uint16_t* __restrict__ k_gamma;
+  const void* __restrict__ table;
+  int32_t ldx, ldw, in, n_total, seq_len, seq_pad, heads, tiles_m, chunk;
+  float eps;
+};
+
+template <bool kOut>
+__device__ __forceinline__ ProjMx4Args unpack(const ProjMx4Packed& p) {
+  ProjMx4Args a{};
+  a.x = p.x, a.w = p.w, a.x_scale = p.x_scale, a.w_scale = p.w_scale;
+  a.ldx = p.ldx, a.ldw = p.ldw, a.in = p.in, a.n_total = p.n_total;
+  a.out.q_out = p.q_out;
+  a.out.seq_len = p.seq_len, a.out.tiles_m = p.tiles_m, a.out.chunk = p.chunk;
+  if constexpr (kOut) {
+    a.out.ldo = p.ldo, a.out.n_out = p.n_total;
+  } else {
+    a.out.k_out = p.k_out, a.out.v_out = p.v_out;
+    a.out.q_gamma = p.q_gamma, a.out.k_gamma = p.k_gamma, a.out.table = p.table;
+    a.out.eps = p.eps, a.out.seq_pad = p.seq_pad, a.out.heads = p.heads;
+  }
+  return a;
+}
+
 template <int kNA, int kMB, bool kPair, int kMode, int kHl, bool kPlain, bool kOut>
-__global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(ProjMx4Args a) {
+__global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(ProjMx4Packed p) {
+  const ProjMx4Args a = unpack<kOut>(p);
   using S = Shape<kNA, kMB, kPair>;
   constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
   static_assert(kChannels < 128 || S::kLds >= 2 * kTokens * kChannels + kWaves * kRowTableLds,
@@ -182,13 +220,22 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(
                                                                    lane2, m0, n0);
 }
 
-// The launch order of a shape's tiles, into a, and the grid that runs it.
+// The kernel's arguments with the launch order of a shape's tiles, and the grid that runs it.
 template <int kNA, int kMB>
-dim3 order_grid(ProjMx4Args& a) {
+ProjMx4Packed pack_args(const ProjMx4Args& a, bool out, dim3& grid) {
   const ProjGrid g = proj_mx4_grid(a.out.seq_len, a.n_total, 32 * kMB, 32 * kNA);
-  a.out.tiles_m = g.order.tiles_m;
-  a.out.chunk = g.order.chunk;
-  return dim3(kOrderXcds * g.longest);
+  grid = dim3(kOrderXcds * g.longest);
+  ProjMx4Packed p{};
+  p.x = a.x, p.w = a.w, p.x_scale = a.x_scale, p.w_scale = a.w_scale;
+  p.q_out = a.out.q_out, p.k_out = a.out.k_out;
+  if (out) p.ldo = a.out.ldo;
+  else p.v_out = a.out.v_out;
+  p.q_gamma = a.out.q_gamma, p.k_gamma = a.out.k_gamma, p.table = a.out.table;
+  p.ldx = (int32_t)a.ldx, p.ldw = (int32_t)a.ldw;      // below 2^23: check_operands()
+  p.in = a.in, p.n_total = a.n_total;
+  p.seq_len = a.out.seq_len, p.seq_pad = a.out.seq_pad, p.heads = a.out.heads;
+  p.tiles_m = g.order.tiles_m, p.chunk = g.order.chunk, p.eps = a.out.eps;
+  return p;
 }
 
 inline int too_large(const ProjMx4Args& a) {

@@ -7,13 +7,14 @@ namespace h3hip {
 namespace {
 
 template <int kNA, int kMB, bool kPair>
-int launch(ProjMx4Args a, hipStream_t st) {
-  const dim3 grid = order_grid<kNA, kMB>(a);
+int launch(const ProjMx4Args& a, hipStream_t st) {
+  dim3 grid;
+  const ProjMx4Packed p = pack_args<kNA, kMB>(a, false, grid);
   constexpr int kOnce = H3HIP_ROUND_ONCE;
   if (a.out.rot == 128)
-    proj_mx4_gemm_kernel<kNA, kMB, kPair, kOnce, 8, false, false><<<grid, kThreads, 0, st>>>(a);
+    proj_mx4_gemm_kernel<kNA, kMB, kPair, kOnce, 8, false, false><<<grid, kThreads, 0, st>>>(p);
   else
-    proj_mx4_gemm_kernel<kNA, kMB, kPair, kOnce, 6, false, false><<<grid, kThreads, 0, st>>>(a);
+    proj_mx4_gemm_kernel<kNA, kMB, kPair, kOnce, 6, false, false><<<grid, kThreads, 0, st>>>(p);
   return check_launch("proj_mx4_gemm_kernel");
 }
 
