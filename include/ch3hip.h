@@ -401,14 +401,15 @@ int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const vo
  *      in_features (up to 33,553,920). w, w_scale: rows of in_features columns as
  *      h3hip_quant_rows_mx4 writes them (padded to a multiple of 256, zeros). y as there.
  *   workspace: device, 16-byte aligned, of at least h3hip_linear_mx4_workspace(rows,
- *      in_features, 0) bytes, of this call alone until it has run (NULL where that is 0).
+ *      in_features) bytes, of this call alone until it has run (NULL where that is 0).
  * Can be captured into a graph. */
 int h3hip_linear_mx4(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* w_scale,
                      int32_t in_features, int32_t out_features, int32_t rows, void* y, int64_t ldy,
                      void* workspace, int64_t workspace_bytes, void* stream);
 
 /* h3hip_qkv_proj_mx4 of bf16 rows in the same way; its workspace is
- * h3hip_linear_mx4_workspace(seq_len, hidden, heads) bytes. */
+ * h3hip_linear_mx4_workspace(seq_len, hidden) bytes. One or two rows take two launches, between
+ * which their fp32 sums lie in the outputs' rows behind them. */
 int h3hip_qkv_linear_mx4(const void* x, int64_t ldx, const void* w, int64_t ldw,
                          const void* w_scale, int32_t hidden, const void* q_gamma,
                          const void* k_gamma, float eps, const void* rope_table, int32_t rot,
@@ -416,8 +417,8 @@ int h3hip_qkv_linear_mx4(const void* x, int64_t ldx, const void* w, int64_t ldw,
                          int32_t head_dim, void* q_out, void* k_out, void* v_out, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace of such a call (heads 0: h3hip_linear_mx4). */
-int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features, int32_t heads);
+/* Bytes of workspace of such a call; 0 for the one or two rows of one launch's product. */
+int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features);
 
 /* ---------------------------------- norm, modulation, gate and residual */
 

@@ -9,11 +9,13 @@
 // straight from memory, B the rows' codes from LDS, in v_mfma_scale_f32_16x16x128_f8f6f4 as in
 // proj_mx4_kernel.h. The four sums are added in LDS, in one order.
 //
-// Of Q | K | V, whose head norm needs 128 channels at once, the sums go to a workspace in fp32, and
-// a second launch of a workgroup a head norms, rotates and stores them. Workgroups of whole heads
-// in one launch leave half the CUs idle, whose loads are what W takes: 13.7 us and more of one
-// token x 5,120 x 40 heads, as the tiles of 128 x 32 behind a rounding of their own do (13.4; of a
-// W that no cache holds 17.3).
+// Of Q | K | V, whose head norm needs 128 channels at once, the fp32 sums go where the head's
+// rows behind the tokens end up as zeros, and a second launch of a workgroup a head norms, rotates
+// and stores them. One token x 5,120 x 40 heads takes 12.3 us replayed from a graph, 14.1 of a W that
+// no cache holds. Workgroups of 16 waves and whole heads, all of W in flight, need one launch and
+// leave half the CUs idle, whose loads are what W takes: 14.4 and 17.0 (host included, where the
+// second launch counts, 13.9 instead of 15.9); the tiles of 128 x 32 behind a rounding of their
+// own take 13.4 and 17.3.
 #include <algorithm>
 
 #include "few_mx4.h"
@@ -44,7 +46,14 @@ inline int64_t lds_bytes(int rows, int units, int hold) {
 constexpr int64_t kMaxLds = 65536;
 inline int hold_of(int units) { return std::min((units + kWaves - 1) / kWaves, kMaxHold); }
 
-// kHold units of a wave in flight; kSums: fp32 sums to a.sums instead of bf16 to a.y.
+// kHold units of a wave in flight; kSums: fp32 sums to the heads instead of bf16 to y.
+// The fp32 sums of a head's rows, [rows][128], from its row kMaxRows on: rows that are behind the
+// last token (seq_pad is a multiple of 128), which few_heads_kernel clears.
+__device__ __forceinline__ float* few_sums(uint16_t* head) {
+  static_assert(3 * kMaxRows <= 128, "the sums fit behind the tokens");
+  return reinterpret_cast<float*>(head + kMaxRows * 128);
+}
+
 template <int kHold, bool kSums>
 __global__ __launch_bounds__(kThreads) void few_mx4_kernel(FewMx4Args a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -156,7 +165,7 @@ __global__ __launch_bounds__(kThreads) void few_mx4_kernel(FewMx4Args a) {
     for (int s = 0; s < kWaves; s++) y += sums[(s * rows + r) * kSumStride + c];
     if (n0 + c < a.n_total) {
       if constexpr (kSums)
-        a.sums[r * (int64_t)a.n_total + n0 + c] = y;
+        few_sums(head_rows(a, n0 / 128))[128 * r + n0 % 128 + c] = y;
       else
         a.y[r * a.ldy + n0 + c] = (uint16_t)(pack_bf16x2(y, y) & 0xffffu);
     }
@@ -166,35 +175,30 @@ __global__ __launch_bounds__(kThreads) void few_mx4_kernel(FewMx4Args a) {
 // What it needs of ProjArgs: a launch of 128 bytes of arguments and more takes the host 0.9 us
 // longer.
 struct FewHeadsArgs {
-  const float* __restrict__ sums;
   const uint16_t* __restrict__ q_gamma;
   const uint16_t* __restrict__ k_gamma;
   const void* __restrict__ table;
-  uint16_t* __restrict__ q_out;
-  uint16_t* __restrict__ k_out;
-  uint16_t* __restrict__ v_out;
+  uint16_t* q_out;
+  uint16_t* k_out;
+  uint16_t* v_out;
   float eps;
   int32_t seq_len, seq_pad, heads;
 };
 
-// Sums [rows, 3 * heads * 128] in fp32 to the heads: a workgroup a head, 8 lanes a row in the
-// prologue's layout, and zeros into the rows behind the last. kPlain: no norm and rotation.
+// The heads of the sums that they hold: a workgroup a head, 8 lanes a row in the prologue's layout,
+// and zeros into the rows behind the last. kPlain: no norm and rotation.
 template <int kMode, int kHl, bool kPlain>
-__global__ __launch_bounds__(kThreads) void few_heads_kernel(FewHeadsArgs a) {
-  const float* __restrict__ sums = a.sums;
-  ProjArgs o{};
-  o.q_gamma = a.q_gamma, o.k_gamma = a.k_gamma, o.table = a.table;
-  o.q_out = a.q_out, o.k_out = a.k_out, o.v_out = a.v_out;
-  o.eps = a.eps, o.seq_len = a.seq_len, o.seq_pad = a.seq_pad, o.heads = a.heads;
+__global__ __launch_bounds__(kThreads) void few_heads_kernel(FewHeadsArgs o) {
   constexpr bool kFull = kHl == 8;
   const int head = (int)blockIdx.x, part = head / o.heads;
   const int row = (int)threadIdx.x >> 3, j = (int)threadIdx.x & 7;
+  const bool pair_lane = kFull || j < kHl;
+  const int chunk_a = pair_lane ? j : 2 * kHl + 2 * (j - kHl);
+  const int chunk_b = pair_lane ? j + kHl : chunk_a + 1;
+  uint16_t* rows = head_rows(o, head);
   if (row < o.seq_len) {
-    const bool pair_lane = kFull || j < kHl;
-    const int chunk_a = pair_lane ? j : 2 * kHl + 2 * (j - kHl);
-    const int chunk_b = pair_lane ? j + kHl : chunk_a + 1;
-    const float* src = sums + ((int64_t)row * 3 * o.heads + head) * 128;
     float v[16];
+    const float* src = few_sums(rows) + 128 * row;
 #pragma unroll
     for (int h = 0; h < 4; h++) {
       const f32x4 t = *reinterpret_cast<const f32x4*>(src + 8 * (h < 2 ? chunk_a : chunk_b) +
@@ -225,10 +229,11 @@ __global__ __launch_bounds__(kThreads) void few_heads_kernel(FewHeadsArgs a) {
       }
       norm_rope<kMode, kFull>(v, gam, pair_lane, tab, o.eps, oa, ob);
     }
-    uint16_t* dst = head_rows(o, head) + (int64_t)row * 128;
+    uint16_t* dst = rows + row * 128;
     *reinterpret_cast<u32x4*>(dst + 8 * chunk_a) = oa;
     *reinterpret_cast<u32x4*>(dst + 8 * chunk_b) = ob;
   }
+  __syncthreads();                         // the sums are read before zeros take their place
   zero_rows<128, kThreads>(o, (int)threadIdx.x, o.seq_len, 128 * head);
 }
 
@@ -236,7 +241,7 @@ template <int kHold>
 void launch(const FewMx4Args& a, hipStream_t st) {
   const dim3 grid((unsigned)(((int64_t)a.n_total + kChannels - 1) / kChannels));
   const size_t lds = lds_bytes(a.rows, a.units, kHold);
-  if (a.sums)
+  if (a.k_out)
     few_mx4_kernel<kHold, true><<<grid, kThreads, lds, st>>>(a);
   else
     few_mx4_kernel<kHold, false><<<grid, kThreads, lds, st>>>(a);
@@ -266,13 +271,12 @@ int launch_few_mx4(const FewMx4Args& a, hipStream_t st) {
   return check_launch("few_mx4_kernel");
 }
 
-int launch_few_heads(const float* sums, const ProjArgs& o, int32_t rounding, bool plain,
-                     hipStream_t st) {
+int launch_few_heads(const ProjArgs& o, int32_t rounding, bool plain, hipStream_t st) {
   constexpr int kRef = H3HIP_ROUND_REFERENCE, kF32 = H3HIP_ROUND_FP32, kOnce = H3HIP_ROUND_ONCE;
   const dim3 grid((unsigned)(3 * o.heads));
   const bool full = o.rot == 128;
-  const FewHeadsArgs a{sums,    o.q_gamma, o.k_gamma, o.table, o.q_out,
-                       o.k_out, o.v_out,   o.eps,     o.seq_len, o.seq_pad, o.heads};
+  const FewHeadsArgs a{o.q_gamma, o.k_gamma, o.table,   o.q_out,   o.k_out,
+                       o.v_out,   o.eps,     o.seq_len, o.seq_pad, o.heads};
   if (plain)
     few_heads_kernel<kRef, 8, true><<<grid, kThreads, 0, st>>>(a);
   else if (rounding == kRef && full)

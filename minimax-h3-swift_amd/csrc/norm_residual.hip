@@ -225,9 +225,12 @@ void norm_residual_kernel(NormArgs<kMany> a) {
     }
   };
   int until = first;                       // the row at which the tables change
-  if constexpr (!kMany) load_tables(0);
+  // Of one segment; beside the next row's loads it would take two registers too many here.
+  if (!kMany && !kAhead) load_tables(0);
   for (int row = first; row < last; row++) {
-    if constexpr (kMany) {
+    if constexpr (!kMany) {
+      if (kAhead && row == first) load_tables(0);
+    } else {
       if (row >= until) {
         int s = 0;
         until = INT_MAX;

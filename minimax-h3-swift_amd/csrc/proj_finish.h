@@ -25,8 +25,8 @@ namespace h3hip {
 // 16-byte chunk c of a head's row l sits at c ^ (l & 15): the 16 rows that a block's write
 // covers, and the two rows x 8 lanes of a read, are on 16 different chunks of a 256-byte bank
 // window each.
-template <int kNA, int kMB, int kLds, int kWaves, int kHl, class Sums>
-__device__ __forceinline__ void finish_tile_once(const ProjArgs& o, float* lds, const Sums& sums,
+template <int kNA, int kMB, int kLds, int kWaves, int kHl, class Args, class Sums>
+__device__ __forceinline__ void finish_tile_once(const Args& o, float* lds, const Sums& sums,
                                                  int wave, int lane, int m0, int n0) {
   constexpr int kChannels = 32 * kNA, kHead = 128, kHeads = kChannels / kHead;
   constexpr int kBlockLds = 32 * kChannels * (int)sizeof(float);
@@ -132,8 +132,8 @@ __device__ __forceinline__ void finish_tile_once(const ProjArgs& o, float* lds, 
 // whose few rows gain nothing from that, are stored from the accumulators, 32 bytes of a
 // row at a time.
 template <int kNA, int kMB, int kLds, int kWaves, int kMode, int kHl, bool kPlain, bool kOut,
-          class Sums>
-__device__ __forceinline__ void finish_tile(const ProjArgs& o, int n_total, uint16_t* lds,
+          class Args, class Sums>
+__device__ __forceinline__ void finish_tile(const Args& o, int n_total, uint16_t* lds,
                                             const Sums& sums, int wave, int lane, int m0, int n0) {
   constexpr int kThreads = 64 * kWaves;
   auto block = [&](int na, int mb) __attribute__((always_inline)) {   // rounded to bf16

@@ -139,7 +139,7 @@ int64_t code_bytes(int32_t rows, int32_t in) { return (int64_t)rows * (padded(in
 int linear(const ProjArgs& o, const void* x, int64_t ldx, const void* w, int64_t ldw,
            const void* w_scale, int32_t in, int32_t n_total, int32_t rounding, bool plain, bool out,
            void* workspace, int64_t workspace_bytes, void* stream) {
-  const int64_t need = h3hip_linear_mx4_workspace(o.seq_len, in, out ? 0 : o.heads);
+  const int64_t need = h3hip_linear_mx4_workspace(o.seq_len, in);
   H3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
              H3HIP_EINVAL, "a workspace of %lld bytes, 16-byte aligned, is needed (%lld given)",
              (long long)need, (long long)(workspace ? workspace_bytes : 0));
@@ -147,14 +147,17 @@ int linear(const ProjArgs& o, const void* x, int64_t ldx, const void* w, int64_t
   H3_REQUIRE(proj_mx4_fits(o.seq_len, n_total, kProjMx4Shapes[0]), H3HIP_EINVAL,
              "too many rows or channels for one launch (%d x %d)", o.seq_len, n_total);
   if (few_mx4_takes(o.seq_len, in)) {
-    float* sums = out ? nullptr : static_cast<float*>(workspace);
-    const int rc = launch_few_mx4(
-        FewMx4Args{static_cast<const uint16_t*>(x), static_cast<const uint8_t*>(w),
-                   static_cast<const uint8_t*>(w_scale), o.q_out, sums, ldx, ldw, o.ldo, o.seq_len,
-                   in, (int32_t)(padded(in) / 256), n_total},
-        as_stream(stream));
+    FewMx4Args few{};
+    few.x = static_cast<const uint16_t*>(x);
+    few.w = static_cast<const uint8_t*>(w);
+    few.w_scale = static_cast<const uint8_t*>(w_scale);
+    few.q_out = o.q_out, few.k_out = o.k_out, few.v_out = o.v_out;
+    few.ldx = ldx, few.ldw = ldw, few.ldy = o.ldo;
+    few.rows = o.seq_len, few.cols = in, few.units = (int32_t)(padded(in) / 256);
+    few.n_total = n_total, few.heads = o.heads, few.seq_pad = o.seq_pad;
+    const int rc = launch_few_mx4(few, as_stream(stream));
     if (rc != H3HIP_OK || out) return rc;
-    return launch_few_heads(sums, o, rounding, plain, as_stream(stream));
+    return launch_few_heads(o, rounding, plain, as_stream(stream));
   }
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scale = codes + code_bytes(o.seq_len, in);
@@ -214,10 +217,8 @@ extern "C" int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scal
                  !q_gamma && !k_gamma, false, stream);
 }
 
-extern "C" int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features, int32_t heads) {
-  if (rows <= 0 || in_features <= 0) return 0;
-  if (few_mx4_takes(rows, in_features))
-    return heads > 0 ? (int64_t)rows * heads * (3 * kHeadDim * sizeof(float)) : 0;
+extern "C" int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features) {
+  if (rows <= 0 || in_features <= 0 || few_mx4_takes(rows, in_features)) return 0;
   const int64_t slabs = ((int64_t)in_features + 511) / 512, groups = ((int64_t)rows + 15) / 16;
   return code_bytes(rows, in_features) + 256 * slabs * groups;
 }

@@ -103,8 +103,8 @@ __device__ __forceinline__ f32x4 block_sums(const f32x32 (&c)[kAccs<kNA, kMB>], 
   return y;
 }
 
-// A ProjMx4Args as the kernel takes it: a launch of 128 bytes of arguments and more takes the host
-// 0.9 us longer.
+// A ProjMx4Args as the kernel and its epilogue take it: a launch of 128 bytes of arguments and
+// more takes the host 0.9 us longer.
 struct ProjMx4Packed {
   const uint8_t* __restrict__ x;
   const uint8_t* __restrict__ w;
@@ -119,30 +119,12 @@ struct ProjMx4Packed {
   const uint16_t* __restrict__ q_gamma;
   const uint16_t* __restrict__ k_gamma;
   const void* __restrict__ table;
-  int32_t ldx, ldw, in, n_total, seq_len, seq_pad, heads, tiles_m, chunk;
+  int32_t ldx, ldw, in, n_out, seq_len, seq_pad, heads, tiles_m, chunk;
   float eps;
 };
 
-template <bool kOut>
-__device__ __forceinline__ ProjMx4Args unpack(const ProjMx4Packed& p) {
-  ProjMx4Args a{};
-  a.x = p.x, a.w = p.w, a.x_scale = p.x_scale, a.w_scale = p.w_scale;
-  a.ldx = p.ldx, a.ldw = p.ldw, a.in = p.in, a.n_total = p.n_total;
-  a.out.q_out = p.q_out;
-  a.out.seq_len = p.seq_len, a.out.tiles_m = p.tiles_m, a.out.chunk = p.chunk;
-  if constexpr (kOut) {
-    a.out.ldo = p.ldo, a.out.n_out = p.n_total;
-  } else {
-    a.out.k_out = p.k_out, a.out.v_out = p.v_out;
-    a.out.q_gamma = p.q_gamma, a.out.k_gamma = p.k_gamma, a.out.table = p.table;
-    a.out.eps = p.eps, a.out.seq_pad = p.seq_pad, a.out.heads = p.heads;
-  }
-  return a;
-}
-
 template <int kNA, int kMB, bool kPair, int kMode, int kHl, bool kPlain, bool kOut>
-__global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(ProjMx4Packed p) {
-  const ProjMx4Args a = unpack<kOut>(p);
+__global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(ProjMx4Packed a) {
   using S = Shape<kNA, kMB, kPair>;
   constexpr int kTokens = 32 * kMB, kChannels = 32 * kNA;
   static_assert(kChannels < 128 || S::kLds >= 2 * kTokens * kChannels + kWaves * kRowTableLds,
@@ -153,7 +135,7 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wc = wave >> 1, wt = wave & 1;   // channel and token half of the tile
-  const TileOrder order{a.out.tiles_m, (a.n_total + kChannels - 1) / kChannels, a.out.chunk};
+  const TileOrder order{a.tiles_m, (a.n_out + kChannels - 1) / kChannels, a.chunk};
   const int xcd = blockIdx.x % kOrderXcds, slot = blockIdx.x / kOrderXcds;
   if (slot >= order.length(xcd)) return;
   const uint32_t tile = order.tile(xcd, slot);
@@ -170,7 +152,7 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(
       ra[2 * b + u] = at + (16 * kNA * wc + lr) * 128;
       rb[2 * b + u] = at + (16 * kMB * wt + lr) * 128;
     }
-  const int ldx = (int)a.ldx, ldw = (int)a.ldw;
+  const int ldx = a.ldx, ldw = a.ldw;
   auto load_offset = [&](int rows, int i, int ld) __attribute__((always_inline)) {
     const int r = rows * wave + 8 * i + (lane >> 3);
     return r * ld + (((lane & 7) ^ p_swz(r)) * 16) - 1024 * (i & 3);
@@ -179,14 +161,14 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(
   for (int i = 0; i < kMB; i++) xv[i] = load_offset(8 * kMB, i, ldx);
 #pragma unroll
   for (int i = 0; i < kNA; i++) wv[i] = load_offset(8 * kNA, i, ldw);
-  const uint64_t xp = (uint64_t)(uintptr_t)(a.x + (int64_t)m0 * a.ldx);
-  const uint64_t wp = (uint64_t)(uintptr_t)(a.w + (int64_t)n0 * a.ldw);
+  const uint64_t xp = (uint64_t)(uintptr_t)(a.x + (int64_t)m0 * ldx);
+  const uint64_t wp = (uint64_t)(uintptr_t)(a.w + (int64_t)n0 * ldw);
   // Bytes of the tile's rows that exist: what lies past them reads as zero.
-  const int x_rows = min(a.out.seq_len - m0, kTokens), w_rows = min(a.n_total - n0, kChannels);
+  const int x_rows = min(a.seq_len - m0, kTokens), w_rows = min(a.n_out - n0, kChannels);
   const int bytes = a.in / 2;
   // The scales of this wave's rows begin at a block of 16 of them; past the last block they
   // read as zeros, which stand for 2^-127.
-  const int x_blocks = (a.out.seq_len + 15) / 16, w_blocks = (a.n_total + 15) / 16;
+  const int x_blocks = (a.seq_len + 15) / 16, w_blocks = (a.n_out + 15) / 16;
   const int x_block = m0 / 16 + kMB * wt, w_block = n0 / 16 + kNA * wc;
   const uint64_t xsp = (uint64_t)(uintptr_t)(a.x_scale + 256 * (int64_t)x_block);
   const uint64_t wsp = (uint64_t)(uintptr_t)(a.w_scale + 256 * (int64_t)w_block);
@@ -216,7 +198,7 @@ __global__ __launch_bounds__(kThreads, kPair ? 2 : 1) void proj_mx4_gemm_kernel(
   auto sums = [&](int na, int mb) __attribute__((always_inline)) {
     return block_sums<kNA, kMB>(c, na, mb);
   };
-  finish_tile<kNA, kMB, S::kLds, kWaves, kMode, kHl, kPlain, kOut>(a.out, a.n_total, lds, sums, wave,
+  finish_tile<kNA, kMB, S::kLds, kWaves, kMode, kHl, kPlain, kOut>(a, a.n_out, lds, sums, wave,
                                                                    lane2, m0, n0);
 }
 
@@ -232,7 +214,7 @@ ProjMx4Packed pack_args(const ProjMx4Args& a, bool out, dim3& grid) {
   else p.v_out = a.out.v_out;
   p.q_gamma = a.out.q_gamma, p.k_gamma = a.out.k_gamma, p.table = a.out.table;
   p.ldx = (int32_t)a.ldx, p.ldw = (int32_t)a.ldw;      // below 2^23: check_operands()
-  p.in = a.in, p.n_total = a.n_total;
+  p.in = a.in, p.n_out = a.n_total;
   p.seq_len = a.out.seq_len, p.seq_pad = a.out.seq_pad, p.heads = a.out.heads;
   p.tiles_m = g.order.tiles_m, p.chunk = g.order.chunk, p.eps = a.out.eps;
   return p;

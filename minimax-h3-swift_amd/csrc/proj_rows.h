@@ -23,15 +23,16 @@ __device__ __forceinline__ void store_row_chunk(uint16_t* dst, u32x4 v, int left
 }
 
 // Head hg of Q | K | V: its part's output, at the head.
-__device__ __forceinline__ uint16_t* head_rows(const ProjArgs& a, int hg) {
+template <class Args>
+__device__ __forceinline__ uint16_t* head_rows(const Args& a, int hg) {
   const int part = hg / a.heads;
   uint16_t* out = part == 0 ? a.q_out : part == 1 ? a.k_out : a.v_out;
   return out + (int64_t)(hg - part * a.heads) * a.seq_pad * 128;
 }
 
 // Zeros into rows m0 .. seq_pad - 1 of the heads of channels n0 .., by kThreads threads.
-template <int kChannels, int kThreads>
-__device__ __forceinline__ void zero_rows(const ProjArgs& a, int tid, int m0, int n0) {
+template <int kChannels, int kThreads, class Args>
+__device__ __forceinline__ void zero_rows(const Args& a, int tid, int m0, int n0) {
   constexpr int kHead = 128, kChunks = kHead / 8;
 #pragma unroll 1
   for (int hg = n0 / kHead; hg < min((n0 + kChannels) / kHead, 3 * a.heads); hg++) {
@@ -119,8 +120,8 @@ constexpr int kRowTableLds = 8 * 64 * sizeof(RopeEntry);   // bytes of a wave
 // the last of one part and the first of the next, or only one. tables: kRowTableLds bytes
 // for each wave.
 template <int kTokens, int kChannels, int kRowWaves, int kMode, int kHl, bool kPlain, bool kOut,
-          bool kAnyWidth = false>
-__device__ __forceinline__ void finish_tile_rows(const ProjArgs& a, const uint16_t* lds,
+          bool kAnyWidth = false, class Args>
+__device__ __forceinline__ void finish_tile_rows(const Args& a, const uint16_t* lds,
                                                  RopeEntry* tables, int wave, int lane, int m0,
                                                  int n0) {
   constexpr int kHead = 128;

@@ -152,8 +152,7 @@ SIGNATURES = {
                                             ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                             ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _vp,
                                             _vp, _vp, _vp, ctypes.c_int64, _vp]),
-    "h3hip_linear_mx4_workspace": (ctypes.c_int64, [ctypes.c_int32, ctypes.c_int32,
-                                                    ctypes.c_int32]),
+    "h3hip_linear_mx4_workspace": (ctypes.c_int64, [ctypes.c_int32, ctypes.c_int32]),
     "h3hip_norm_modulate": (ctypes.c_int, [_vp, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
                                            ctypes.POINTER(NormC), ctypes.c_float, _i32p,
                                            ctypes.c_int32, _vp, ctypes.c_int64, _vp]),

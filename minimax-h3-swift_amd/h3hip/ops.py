@@ -604,8 +604,8 @@ def dequant_rows_mx4(rows: Mx4Rows, out: torch.Tensor | None = None) -> torch.Te
 
 
 @functools.lru_cache(maxsize=1024)
-def _mx4_workspace(S: int, K: int, heads: int) -> int:
-    return L.lib().h3hip_linear_mx4_workspace(S, K, heads)
+def _mx4_workspace(S: int, K: int) -> int:
+    return L.lib().h3hip_linear_mx4_workspace(S, K)
 
 
 def _mx4_operands(x, w):
@@ -666,7 +666,7 @@ def proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, out: torch.Tensor | None = N
         rc = _run(L.lib().h3hip_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
                   v.data_ptr(), ldw, s.data_ptr(), 2 * v.shape[1], N, S, out.data_ptr(), ldy)
     else:
-        size, work = _mx4_workspace(S, K, 0), None
+        size, work = _mx4_workspace(S, K), None
         if size:
             work = _empty(size, dtype=_U8, device=device)
         rc = _run(L.lib().h3hip_linear_mx4, device, x.data_ptr(), ldx, v.data_ptr(), ldw,
@@ -707,7 +707,7 @@ def qkv_proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, q_gamma: torch.Tensor | 
         rc = _run(L.lib().h3hip_qkv_proj_mx4, device, x.values.data_ptr(), ldx, x.scale.data_ptr(),
                   v.data_ptr(), ldw, s.data_ptr(), 2 * v.shape[1], *norm)
     else:
-        size, work = _mx4_workspace(S, K, heads), None
+        size, work = _mx4_workspace(S, K), None
         if size:
             work = _empty(size, dtype=_U8, device=device)
         rc = _run(L.lib().h3hip_qkv_linear_mx4, device, x.data_ptr(), ldx, v.data_ptr(), ldw,

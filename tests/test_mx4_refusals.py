@@ -121,23 +121,22 @@ def test_linear(h3, bad, word):
     (dict(k=0), "hidden"), (dict(S=0), "shape"), (dict(H=0), "shape"), (dict(pad=64), "shape"),
     (dict(gq=None), "gammas"), (dict(table=None), "table"), (dict(rounding=2), "rounding"),
     (dict(q=None), "NULL"), (dict(v=at(8)), "aligned"), (dict(size=4 * 256 + 255), "workspace"),
-    (dict(S=2, k=504, ldx=504, size=2 * 2 * 1536 - 1), "workspace")])
+    (dict(S=2, size=2 * 256 + 255), "workspace")])
 def test_qkv_linear(h3, bad, word):
     from h3hip import _lib
     assert _qkv_linear(h3, **bad) == _lib.EINVAL and word in h3.last_error()
 
 
 def test_linear_workspace(h3):
-    """Codes and scales of the rows, or the sums of one or two rows' heads; none for their
-    token-major product, nor where there is nothing to do."""
+    """Codes and scales of the rows; none for one or two rows, nor where there is nothing to do."""
     from h3hip import _lib
     size = h3.lib().h3hip_linear_mx4_workspace
-    assert size(4, 500, 0) == size(4, 500, 7) == 4 * 256 + 256
-    assert size(100, 5120, 0) == 100 * 2560 + 10 * 7 * 256
-    assert size(2, 504, 0) == 0 and size(2, 504, 3) == 2 * 3 * 384 * 4
-    assert size(2, 500, 0) == 2 * 256 + 256        # not a multiple of 8 columns
-    assert size(2, 200_000, 0) == 2 * 100_096 + 391 * 256    # codes past the LDS
-    assert size(0, 500, 0) == size(4, 0, 0) == size(-1, -1, -1) == 0
+    assert size(4, 500) == 4 * 256 + 256
+    assert size(100, 5120) == 100 * 2560 + 10 * 7 * 256
+    assert size(1, 8) == size(2, 504) == 0
+    assert size(2, 500) == 2 * 256 + 256        # not a multiple of 8 columns
+    assert size(2, 200_000) == 2 * 100_096 + 391 * 256    # codes past the LDS
+    assert size(0, 500) == size(4, 0) == size(-1, -1) == 0
     assert _linear(h3, rows=0, x=None, y=None, work=None, size=0) == _lib.OK
     for bad in (dict(D=64), dict(rot=64)):
         assert _qkv_linear(h3, **bad) == _lib.DECLINED and "declined" in h3.last_error()
