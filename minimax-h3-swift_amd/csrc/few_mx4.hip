@@ -11,10 +11,10 @@
 //
 // Of Q | K | V, whose head norm needs 128 channels at once, the fp32 sums go where the head's
 // rows behind the tokens end up as zeros, and a second launch of a workgroup a head norms, rotates
-// and stores them. One token x 5,120 x 40 heads takes 12.3 us replayed from a graph, 14.1 of a W that
+// and stores them. One token x 5,120 x 40 heads takes 12.4 us replayed from a graph, 14.0 of a W that
 // no cache holds. Workgroups of 16 waves and whole heads, all of W in flight, need one launch and
 // leave half the CUs idle, whose loads are what W takes: 14.4 and 17.0 (host included, where the
-// second launch counts, 13.9 instead of 15.9); the tiles of 128 x 32 behind a rounding of their
+// second launch counts, 13.9 instead of 15.8); the tiles of 128 x 32 behind a rounding of their
 // own take 13.4 and 17.3.
 #include <algorithm>
 

@@ -10,7 +10,7 @@
 // from the rounded one.
 //
 // Bound by HBM: before 4 bytes an element, after with a next norm 8 (31,885 x 5,120: 137 us, 4.8
-// TB/s, and 265 us, 4.9; a copy of 1 GiB 5.1), of few rows by the launch (125 x 5,120: 4.2 us). So a
+// TB/s, and 264 us, 4.9; a copy of 1 GiB 5.1), of few rows by the launch (125 x 5,120: 3.8 us). So a
 // row is read once and stays in registers through its sums, and the tables, which as rows are as long as x's, are held
 // in registers too, by workers that take a range of consecutive rows each and reload the
 // tables only where a segment begins. The next row's loads are in flight while one is summed (of
@@ -33,7 +33,7 @@ constexpr int kMaxThreads = 1024;
 constexpr int kMaxHidden = 2 * kMaxThreads * kLaneElems;
 constexpr int kCus = 256;
 // Waves a CU: 6 a SIMD in 80 registers. In the 94 that the compiler took by itself two workgroups of
-// 11 waves did not fit a CU (31,885 x 5,376, after with a next norm, 373 us; 290).
+// 11 waves did not fit a CU (31,885 x 5,376, after with a next norm, 373 us; 297).
 constexpr int kWavesCu = 24;
 
 // What a launch needs where one segment holds every row: 120 bytes, because the host takes 0.9 us
