@@ -399,7 +399,9 @@ int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const vo
  * product's launch, whose sums add in another order.
  *   x: device bf16 [rows, in_features], row stride ldx elements; rows may begin anywhere; any
  *      in_features (up to 33,553,920). w, w_scale: rows of in_features columns as
- *      h3hip_quant_rows_mx4 writes them (padded to a multiple of 256, zeros). y as there.
+ *      h3hip_quant_rows_mx4 writes them (padded to a multiple of 256, zeros). y as there; of
+ *      one or two rows no row of y may overlap one of x (H3HIP_EINVAL): the product's launch
+ *      reads the one while it writes the other.
  *   workspace: device, 16-byte aligned, of at least h3hip_linear_mx4_workspace(rows,
  *      in_features) bytes, of this call alone until it has run (NULL where that is 0).
  * Can be captured into a graph. */
@@ -409,7 +411,8 @@ int h3hip_linear_mx4(const void* x, int64_t ldx, const void* w, int64_t ldw, con
 
 /* h3hip_qkv_proj_mx4 of bf16 rows in the same way; its workspace is
  * h3hip_linear_mx4_workspace(seq_len, hidden) bytes. One or two rows take two launches, between
- * which their fp32 sums lie in the outputs' rows behind them. */
+ * which their fp32 sums lie in the outputs' rows behind them; no output may overlap x then
+ * (H3HIP_EINVAL). */
 int h3hip_qkv_linear_mx4(const void* x, int64_t ldx, const void* w, int64_t ldw,
                          const void* w_scale, int32_t hidden, const void* q_gamma,
                          const void* k_gamma, float eps, const void* rope_table, int32_t rot,

@@ -135,6 +135,27 @@ int product(const ProjArgs& o, const void* x, int64_t ldx, const void* x_scale, 
 // Bytes of the codes of `rows` rows in a workspace; their scales follow.
 int64_t code_bytes(int32_t rows, int32_t in) { return (int64_t)rows * (padded(in) / 2); }
 
+// Whether an output lies on one of the few rows of x, which every workgroup of few_mx4_kernel
+// reads while others store.
+bool on_few_rows(const ProjArgs& o, const void* x, int64_t ldx, int32_t in, int32_t n_total, bool out) {
+  auto meet = [](uintptr_t a, int64_t na, const void* b, int64_t nb) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(b);
+    return a < at + (uintptr_t)nb && at < a + (uintptr_t)na;
+  };
+  for (int32_t r = 0; r < o.seq_len; r++) {
+    const uintptr_t row = reinterpret_cast<uintptr_t>(x) + 2 * (uintptr_t)(r * ldx);
+    if (out) {
+      for (int32_t s = 0; s < o.seq_len; s++)
+        if (meet(row, 2 * (int64_t)in, o.q_out + s * o.ldo, 2 * (int64_t)n_total)) return true;
+    } else {
+      const int64_t heads = 2 * (int64_t)o.heads * o.seq_pad * kHeadDim;
+      for (const uint16_t* t : {o.q_out, o.k_out, o.v_out})
+        if (meet(row, 2 * (int64_t)in, t, heads)) return true;
+    }
+  }
+  return false;
+}
+
 // The product of bf16 rows: one or two rounded on the way, more into the workspace first.
 int linear(const ProjArgs& o, const void* x, int64_t ldx, const void* w, int64_t ldw,
            const void* w_scale, int32_t in, int32_t n_total, int32_t rounding, bool plain, bool out,
@@ -147,6 +168,8 @@ int linear(const ProjArgs& o, const void* x, int64_t ldx, const void* w, int64_t
   H3_REQUIRE(proj_mx4_fits(o.seq_len, n_total, kProjMx4Shapes[0]), H3HIP_EINVAL,
              "too many rows or channels for one launch (%d x %d)", o.seq_len, n_total);
   if (few_mx4_takes(o.seq_len, in)) {
+    H3_REQUIRE(!on_few_rows(o, x, ldx, in, n_total, out), H3HIP_EINVAL,
+               "an output overlaps x: of one or two rows the product reads x while it is written");
     FewMx4Args few{};
     few.x = static_cast<const uint16_t*>(x);
     few.w = static_cast<const uint8_t*>(w);

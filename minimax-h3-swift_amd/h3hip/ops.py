@@ -651,7 +651,8 @@ def proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, out: torch.Tensor | None = N
     x: [S, K] bf16 (row stride free), rounded as by quant_rows_mx4() on the way, or an
     Mx4Rows; w: [N, K], rounded or laid out once (S and N up to 16,776,960). One or two bf16
     rows take one launch, whose sums add in another order than those of more. Returns y [S, N]
-    bf16 (or writes ``out``, any row stride), or None when declined."""
+    bf16 (or writes ``out``, any row stride; not on top of one or two rows of x), or None when
+    declined."""
     device, S, N, ldx, ldw = _mx4_operands(x, w)
     if out is None:
         out = _empty(S, N, dtype=_BF16, device=device)
