@@ -398,7 +398,7 @@ int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const vo
  * of their own before the product, or, one or two rows (of a multiple of 8 columns), in the
  * product's launch, whose sums add in another order.
  *   x: device bf16 [rows, in_features], row stride ldx elements; rows may begin anywhere; any
- *      in_features (up to 33,553,920). w, w_scale: rows of in_features columns as
+ *      in_features up to 16,776,960 (H3HIP_EINVAL past it). w, w_scale: rows of in_features columns as
  *      h3hip_quant_rows_mx4 writes them (padded to a multiple of 256, zeros). y as there; of
  *      one or two rows no row of y may overlap one of x (H3HIP_EINVAL): the product's launch
  *      reads the one while it writes the other.
@@ -420,7 +420,8 @@ int h3hip_qkv_linear_mx4(const void* x, int64_t ldx, const void* w, int64_t ldw,
                          int32_t head_dim, void* q_out, void* k_out, void* v_out, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace of such a call; 0 for the one or two rows of one launch's product. */
+/* Bytes of workspace of such a call; 0 for the one or two rows of one launch's product, and for more
+ * rows or columns than a call takes (16,776,960 of either). */
 int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features);
 
 /* ---------------------------------- norm, modulation, gate and residual */

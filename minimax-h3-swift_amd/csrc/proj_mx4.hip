@@ -242,6 +242,8 @@ extern "C" int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scal
 
 extern "C" int64_t h3hip_linear_mx4_workspace(int32_t rows, int32_t in_features) {
   if (rows <= 0 || in_features <= 0 || few_mx4_takes(rows, in_features)) return 0;
+  // What every call refuses (check_linear(), linear()).
+  if (padded(in_features) / 2 >= kMaxStride || !proj_mx4_fits(rows, 1, kProjMx4Shapes[0])) return 0;
   const int64_t slabs = ((int64_t)in_features + 511) / 512, groups = ((int64_t)rows + 15) / 16;
   return code_bytes(rows, in_features) + 256 * slabs * groups;
 }

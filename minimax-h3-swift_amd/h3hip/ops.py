@@ -649,7 +649,7 @@ def proj_mx4(x: torch.Tensor | Mx4Rows, w: Mx4Rows, out: torch.Tensor | None = N
     """A projection on 4-bit operands: y = x . w^T with fp32 sums.
 
     x: [S, K] bf16 (row stride free), rounded as by quant_rows_mx4() on the way, or an
-    Mx4Rows; w: [N, K], rounded or laid out once (S and N up to 16,776,960). One or two bf16
+    Mx4Rows; w: [N, K], rounded or laid out once (S, N and K up to 16,776,960). One or two bf16
     rows take one launch, whose sums add in another order than those of more. Returns y [S, N]
     bf16 (or writes ``out``, any row stride; not on top of one or two rows of x), or None when
     declined."""
