@@ -18,10 +18,10 @@
 // A worker is a workgroup of as many waves as the row has chunks of 512 elements (of 1,024 past
 // 8,192): 8 elements a thread. That depends on the width alone, and sums add in one order, so a
 // row's bits do not depend on the other rows of the call.
-#include <algorithm>
 #include <climits>
 
 #include "common.h"
+#include "norm_rule.h"
 
 namespace h3hip {
 
@@ -31,10 +31,6 @@ constexpr int kMaxSegments = 16;
 constexpr int kLaneElems = 8;              // consecutive elements of a thread in a chunk
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxHidden = 2 * kMaxThreads * kLaneElems;
-constexpr int kCus = 256;
-// Waves a CU: 6 a SIMD in 80 registers. In the 94 that the compiler took by itself two workgroups of
-// 11 waves did not fit a CU (31,885 x 5,376, after with a next norm, 373 us; 297).
-constexpr int kWavesCu = 24;
 
 // What a launch needs where one segment holds every row: 120 bytes, because the host takes 0.9 us
 // longer for a launch of 128 bytes of arguments and more (the kernel's use of the launch's
@@ -69,7 +65,7 @@ __host__ __device__ constexpr int waves_of(int hidden) {
   return (hidden + 64 * kLaneElems * kChunks - 1) / (64 * kLaneElems * kChunks);
 }
 __host__ __device__ constexpr int workers_of(int rows, int workers_cu) {
-  const int most = kCus * workers_cu;
+  const int most = kNormCus * workers_cu;
   return rows < most ? rows : most;
 }
 
@@ -141,7 +137,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 // kChunks chunks of a row a thread. kAfter: there is y; kPost: it is normalised; kNext: h is
 // written (without kAfter always); kMany: rows of more than one segment.
 template <int kChunks, bool kAfter, bool kPost, bool kNext, bool kMany>
-__global__ __launch_bounds__(kMaxThreads) __attribute__((amdgpu_waves_per_eu(kChunks == 1 ? 6 : 4)))
+__global__ __launch_bounds__(kMaxThreads)
+__attribute__((amdgpu_waves_per_eu(norm_waves_simd(kChunks, kAfter, kPost, kNext, kMany))))
 void norm_residual_kernel(NormArgs<kMany> a) {
   constexpr int kSums = (kPost ? 1 : 0) + (kNext ? 1 : 0);
   constexpr int kMaxWaves = kMaxThreads / 64;
@@ -298,25 +295,32 @@ void norm_residual_kernel(NormArgs<kMany> a) {
   }
 }
 
-template <int kChunks, bool kMany>
-void launch_chunks(const NormArgs<kMany>& a, hipStream_t st) {
-  const dim3 block(64 * waves_of<kChunks>(a.hidden));
+template <int kChunks, bool kAfter, bool kPost, bool kNext, bool kMany>
+void launch_form(NormArgs<kMany>& a, hipStream_t st) {
+  const int waves = waves_of<kChunks>(a.hidden);
+  a.workers_cu = (uint16_t)norm_workers_cu(
+      waves, a.rows, norm_waves_simd(kChunks, kAfter, kPost, kNext, kMany));
   const dim3 grid((unsigned)workers_of(a.rows, a.workers_cu));
+  norm_residual_kernel<kChunks, kAfter, kPost, kNext, kMany><<<grid, 64 * waves, 0, st>>>(a);
+}
+
+template <int kChunks, bool kMany>
+void launch_chunks(NormArgs<kMany>& a, hipStream_t st) {
   const bool next = a.h != nullptr;
   if (a.y == nullptr)
-    norm_residual_kernel<kChunks, false, false, true, kMany><<<grid, block, 0, st>>>(a);
+    launch_form<kChunks, false, false, true>(a, st);
   else if (a.post && next)
-    norm_residual_kernel<kChunks, true, true, true, kMany><<<grid, block, 0, st>>>(a);
+    launch_form<kChunks, true, true, true>(a, st);
   else if (a.post)
-    norm_residual_kernel<kChunks, true, true, false, kMany><<<grid, block, 0, st>>>(a);
+    launch_form<kChunks, true, true, false>(a, st);
   else if (next)
-    norm_residual_kernel<kChunks, true, false, true, kMany><<<grid, block, 0, st>>>(a);
+    launch_form<kChunks, true, false, true>(a, st);
   else
-    norm_residual_kernel<kChunks, true, false, false, kMany><<<grid, block, 0, st>>>(a);
+    launch_form<kChunks, true, false, false>(a, st);
 }
 
 template <bool kMany>
-void launch(const NormArgs<kMany>& a, hipStream_t st) {
+void launch(NormArgs<kMany>& a, hipStream_t st) {
   if (a.hidden <= kMaxThreads * kLaneElems) launch_chunks<1>(a, st);
   else launch_chunks<2>(a, st);
 }
@@ -324,10 +328,8 @@ void launch(const NormArgs<kMany>& a, hipStream_t st) {
 // Fills in the sizes and launches; a's tables are the first segment's.
 int launch(NormArgs<true>& a, int32_t rows, int32_t hidden, float eps, const int32_t* starts,
            int32_t segments, void* stream) {
-  const int waves = hidden <= kMaxThreads * kLaneElems ? waves_of<1>(hidden) : waves_of<2>(hidden);
   a.rows = rows;
   a.hidden = (uint16_t)hidden;
-  a.workers_cu = (uint16_t)std::max(1, kWavesCu / waves);
   a.eps = eps;
   a.segments = segments;
   for (int i = 1; i < segments; i++) a.starts[i] = starts[i];
