@@ -58,9 +58,9 @@ extern "C" {
 #define H3HIP_ROUND_FP32 1      /* fp32 until the single store */
 #define H3HIP_ROUND_ONCE 3      /* FP32, and the projection's product stays fp32 as well, where
                                    FP32 normalises the bf16 product: one rounding to bf16 from
-                                   the operands to Q and K. h3hip_qkv_proj_i8 and
-                                   h3hip_qkv_proj_mx4 only; h3hip_rope_table writes FP32's
-                                   table for it */
+                                   the operands to Q and K. h3hip_qkv_proj_i8,
+                                   h3hip_qkv_proj_mx4 and h3hip_qkv_linear_mx4 only;
+                                   h3hip_rope_table writes FP32's table for it */
 
 /* Output layouts of the attention. */
 #define H3HIP_OUT_HEAD_MAJOR 0  /* [heads, seq_pad, head_dim] */
@@ -352,7 +352,8 @@ int h3hip_qkv_proj_i8(const void* x, int64_t ldx, const float* x_scale, const vo
  *          and block b's e + 127 (255: NaN) at [b/16][r/16][16*(b%4) + r%16][b/4%4], the order
  *          in which the projections read them. All of it is written, of rows and blocks that
  *          do not exist as 0.
- * rows may be 0; cols at most 33,553,920. No workspace; can be captured into a graph. */
+ * rows may be 0; cols at most 33,553,920. No output of this section may overlap an input, but
+ * where it is said. No workspace; can be captured into a graph. */
 int h3hip_quant_rows_mx4(const void* x, int64_t ldx, int32_t rows, int32_t cols, void* q,
                          int64_t ldq, void* scale, void* stream);
 
@@ -399,9 +400,9 @@ int h3hip_qkv_proj_mx4(const void* x, int64_t ldx, const void* x_scale, const vo
  * product's launch, whose sums add in another order.
  *   x: device bf16 [rows, in_features], row stride ldx elements; rows may begin anywhere; any
  *      in_features up to 16,776,960 (H3HIP_EINVAL past it). w, w_scale: rows of in_features columns as
- *      h3hip_quant_rows_mx4 writes them (padded to a multiple of 256, zeros). y as there; of
- *      one or two rows no row of y may overlap one of x (H3HIP_EINVAL): the product's launch
- *      reads the one while it writes the other.
+ *      h3hip_quant_rows_mx4 writes them (padded to a multiple of 256, zeros). y as there; it may be
+ *      x or overlap it, but of one or two rows no row of y may overlap one of x
+ *      (H3HIP_EINVAL): the product's launch reads the one while it writes the other.
  *   workspace: device, 16-byte aligned, of at least h3hip_linear_mx4_workspace(rows,
  *      in_features) bytes, of this call alone until it has run (NULL where that is 0).
  * Can be captured into a graph. */
@@ -447,8 +448,8 @@ typedef struct {
  *   starts: host, the first row of each segment, not descending, starts[0] = 0; NULL: one
  *      segment. Segments of no rows, and starts past the last row, are fine. Travels by value.
  *   segments: 1 to 16.
- * rows may be 0. A row whose squares pass fp32 (magnitudes of 1e18 and more) comes out as its
- * shift. No workspace; can be captured into a graph. Declines hidden above 16,384. */
+ * rows may be 0. A row whose squares add up past fp32 (a root mean square above 1.8e19 /
+ * sqrt(hidden)) comes out as its shift. No workspace; can be captured into a graph. Declines hidden above 16,384. */
 int h3hip_norm_modulate(const void* x, int64_t ldx, int32_t rows, int32_t hidden,
                         const h3hip_norm* norm, float eps, const int32_t* starts,
                         int32_t segments, void* h, int64_t ldh, void* stream);

@@ -10,7 +10,8 @@
 // from the rounded one.
 //
 // Bound by HBM: before 4 bytes an element, after with a next norm 8 (31,885 x 5,120: 137 us, 4.8
-// TB/s, and 264 us, 4.9; a copy of 1 GiB 5.1), of few rows by the launch (125 x 5,120: 3.8 us). So a
+// TB/s, and 264 us, 4.9; a copy of 1 GiB 5.1; 18,102 rows of 7,168 to 16,384 4.5-5.1 but for 4.2 of
+// 9,000), of few rows by the launch (125 x 5,120: 3.8 us). So a
 // row is read once and stays in registers through its sums, and the tables, which as rows are as long as x's, are held
 // in registers too, by workers that take a range of consecutive rows each and reload the
 // tables only where a segment begins. The next row's loads are in flight while one is summed (of
@@ -146,7 +147,9 @@ void norm_residual_kernel(NormArgs<kMany> a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int n = a.hidden, waves = waves_of<kChunks>(n);
-  // Rows first to last - 1: as many for every worker, one more for the first of them.
+  // Rows first to last - 1: as many for every worker, one more for the first of them. With the one
+  // more spread evenly 18,102 x 5,120 takes 88 us before and 162 after with a next norm instead of 78 and
+  // 152, 31,885 x 5,376 147 and 291 instead of 151 and 293: where in memory the workers stand.
   const uint32_t workers = (uint32_t)workers_of(a.rows, a.workers_cu), rows = (uint32_t)a.rows;
   const uint32_t share = rows / workers, more = rows - share * workers;
   const int first = (int)(blockIdx.x * share + min(blockIdx.x, more));

@@ -20,7 +20,8 @@ namespace h3hip {
 // kBlocks x 32 tokens, the accumulators of the later ones waiting in their registers. Against
 // the bf16 rows of H3HIP_ROUND_FP32 a QKV call of 31,885 x 40 heads x 5,120 takes 0.8% more (2,077
 // us), of 1,151 x 56 heads 0.7%, of one token nothing (int8; on 4-bit operands, whose loop is half as
-// long, 4%: 1,273 -> 1,323 us).
+// long, 4% on 256 x 256: 1,273 -> 1,323 us; on the 256 x 224 that is picked less than nothing, 1,269 ->
+// 1,247 in turn, and 1,124 without norm and rotation).
 //
 // 16-byte chunk c of a head's row l sits at c ^ (l & 15): the 16 rows that a block's write
 // covers, and the two rows x 8 lanes of a read, are on 16 different chunks of a 256-byte bank

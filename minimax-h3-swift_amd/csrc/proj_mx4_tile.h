@@ -79,11 +79,16 @@ inline float proj_mx4_cost(const ProjMx4Shape& s, int tiles, int rounds, int ste
 //
 // The constants were fitted to what they pick: 7,571 sizes of both forms (1 to 32,000 tokens, 200 to
 // 21,504 channels, 1 to 28 steps; heads with norm in H3HIP_ROUND_ONCE) timed on every shape on MI355X.
-// On the 30% of them that the search did not see the pick is 1.2% slower than the best shape on
-// average; with a term in rounds alone, as for int8, whose constants lose 1.6% (3.8% past 2,000
-// tokens), least squares lose 1.7%. Every shape is the pick for 30 of the sizes or more, and
-// without it those take 3-20% longer. 31,885 tokens x 5,120 x 5,120 take 431 us on 256 x 192, 468
-// on 256 x 256 and 538 on 128 x 192; 1,151 x 56 heads x 5,376 77 us on 256 x 192, 88 on 256 x 256.
+// On the 30% of them (2,243) that the search did not see the pick is 1.0% slower than the best shape
+// on average, 1.9% past 2,000 tokens; with int8's constants, a term in rounds alone, 1.6% and 3.8%. Every
+// shape is the pick for 30 of the sizes or more, and without it those take 3-20% longer. A cost
+// ranks shapes and is no time of its own: of nine in ten picks it is 0.79 to 1.16 of the time. Shapes in
+// turn (replays, medians of 7, us; * the pick):
+//   31,885 x 5,120 x 5,120          256 x 256 385, x 224* 399, x 192 405, x 160 420, 128 x 192 542
+//   31,885 x 5,120 x 40 heads       256 x 256 1,224, x 224* 1,246, x 192 1,273, x 160 1,328, 128 x 192 1,507
+//   1,151 x 5,376 x 56 heads        256 x 256 83, x 224 80, x 192* 73, x 160 82, 128 x 192 81
+// Which of the first three is best depends on how warm the chip is: one after another without a
+// pause, on another box, 469, 445, 434; 1,342, 1,294, 1,334; 89, 84, 78.
 inline ProjMx4Tile pick_proj_mx4_tile(int tokens, int channels, int steps, bool heads) {
   float best = 0.f;
   ProjMx4Tile tile = ProjMx4Tile::kNone;
