@@ -14,7 +14,7 @@
 //
 // Epilogue: proj_finish.h, on the sums as they are.
 //
-// What bounds it: large products the chip's power limit (31,885 x 5,120 x 5,120 393-445 us by box
+// What bounds it: large products the chip's power limit (31,885 x 5,120 x 5,120 393-445 us by card
 // and warmth, 3,760 to 4,250 TFLOP/s, matrix cores busy 53% of the cycles at 1.8 GHz; a stream of the instruction alone 7,090; a
 // step of a 256 x 256 tile 1.59 us on Gaussians and 1.31 on zeros), 637 x 1,000 x 777 the latency of its four
 // steps (4.8 us). Two workgroups of 128 x 192 a CU, whose loops cover each other's epilogues, are bound by

@@ -88,7 +88,7 @@ inline float proj_mx4_cost(const ProjMx4Shape& s, int tiles, int rounds, int ste
 //   31,885 x 5,120 x 40 heads       256 x 256 1,224, x 224* 1,246, x 192 1,273, x 160 1,328, 128 x 192 1,507
 //   1,151 x 5,376 x 56 heads        256 x 256 83, x 224 80, x 192* 73, x 160 82, 128 x 192 81
 // Which of the first three is best depends on how warm the chip is: one after another without a
-// pause, on another box, 469, 445, 434; 1,342, 1,294, 1,334; 89, 84, 78.
+// pause, on another card, 469, 445, 434; 1,342, 1,294, 1,334; 89, 84, 78.
 inline ProjMx4Tile pick_proj_mx4_tile(int tokens, int channels, int steps, bool heads) {
   float best = 0.f;
   ProjMx4Tile tile = ProjMx4Tile::kNone;
