@@ -119,8 +119,8 @@ def cpu_baseline(shape, plan_rows, seconds: float = 12.0):
     k = rng.standard_normal((S, D), dtype=np.float32)
     v = rng.standard_normal((S, D), dtype=np.float32)
     model, nproc, avail, omp_env = host_cpu()
-    # Every host CPU this process may run on, at most the 16 that the GPU box
-    # allots to one GPU.
+    # Every host CPU this process may run on, at most 16: one GPU's share
+    # of its node.
     threads = min(16, avail)
 
     rows = np.arange(S, dtype=np.int32)
@@ -844,7 +844,7 @@ def main() -> int:
         # The same rate against the dense bf16 peak at a clock NOT measured in
         # this run: the committed profile's cycles per XCD (GRBM_GUI_ACTIVE)
         # over its unprofiled duration, from an earlier run and possibly another
-        # box. Context only; the roofline fraction is against the spec peak.
+        # card. Context only; the roofline fraction is against the spec peak.
         "attn_profiled_clock_ghz": clk,
         "attn_profiled_clock_source": "profiles/bsattn_fwd_cfg3_clock.txt (an earlier run)",
         "attn_mfma_peak_frac_at_profiled_clock": (

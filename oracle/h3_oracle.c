@@ -1,7 +1,7 @@
 /*
  * h3_oracle.c -- TEST INFRASTRUCTURE, NOT PRODUCT CODE.
  *
- * A CPU restatement of the reference's attention hot path. It is the checker
+ * A CPU restatement of the reference's attention hot path. It is what
  * the HIP library is compared against and the CPU baseline bench.py times;
  * the product never calls into it. Citations are to the reference tree
  * (loading-awesome/MiniMax-H3-Swift).

@@ -2,7 +2,7 @@
  * h3_oracle.h -- TEST INFRASTRUCTURE, NOT PRODUCT CODE.
  *
  * CPU restatement of the reference's DiT attention hot path, used only as the
- * checker: by tests/, by __graft_entry__.smoke() and by bench.py's
+ * oracle: by tests/, by __graft_entry__.smoke() and by bench.py's
  * cpu_baseline leg. Nothing in the shipped library links, loads or calls it.
  *
  * Every function cites the reference file:line it restates (paths relative to
